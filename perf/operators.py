@@ -220,7 +220,7 @@ def prepare(case, seed):
         start = torch.tensor([0] + sizes).cumsum(0).to(torch.int32)
         s.update(q=_randn((sum(sizes), c["hq"], c["dim"]), seed, 4, dt), start=start.cuda(),
                  prefixes=torch.tensor(prefixes, dtype=torch.int32, device="cuda"), largest=max(sizes),
-                 longest=max(prefixes), window=c["window"], sinks=c["sinks"])
+                 window=c["window"], sinks=c["sinks"])
     else:
         rows = _rows_of(c)[0]
         start = torch.tensor([0] + rows).cumsum(0).to(torch.int32)
@@ -258,7 +258,7 @@ def _run_own(s):
                                           max_query_len=s["longest"], **s["kw"])]
     return [iva.paged_prefix_decode_attention(
         s["q"], s["k_pool"], s["v_pool"], s["tables"], s["lens"], s["start"], s["prefixes"], window=s["window"],
-        n_sink=s["sinks"], max_group=s["largest"], max_prefix_len=s["longest"], **s["kw"])]
+        n_sink=s["sinks"], max_group=s["largest"], **s["kw"])]
 
 
 def _page_rows(s, pages):
