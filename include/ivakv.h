@@ -427,6 +427,75 @@ int ivakv_prefill_attn_split_fp8(const void* q, const void* k_pool, const void* 
                                  int dtype, hipStream_t stream);
 
 /*
+ * Cross attention: the rows of sequence b, query_start[b] .. query_start[b+1]-1 of q
+ * [n_tok][Hq][D], attend to all of its keys 0 .. context_lens[b]-1 in the pages (an encoder's
+ * states, say), without a causal mask; out is like q.  Layouts, page rules and max_query_len as
+ * in ivakv_prefill_attn (rows of a sequence past max_query_len, and rows of no sequence, are
+ * left as they are); a row without keys gives zeros.  k_scale / v_scale: the factors of FP8
+ * pools (fp16 or bf16 queries), NULL for pools of the queries' type.  Two launches at most, no
+ * host synchronisation.  The workspace (ivakv_cross_workspace_size; fp8: 1 for FP8 pools) needs no
+ * initialisation; calls that share one must not run concurrently.
+ * Replaces: AttentionTorch.forward with config.causal False (src/core/attention.py:77-102).
+ */
+int ivakv_cross_workspace_size(int batch, int n_tok, int max_query_len, int num_q_heads,
+                               int num_kv_heads, int head_dim, int dtype, int fp8, size_t* bytes);
+int ivakv_cross_attn(const void* q, const void* k_pool, const void* v_pool, const float* k_scale,
+                     const float* v_scale, const int32_t* block_tables, const int32_t* context_lens,
+                     const int32_t* query_start, int n_tok, void* out, void* workspace,
+                     size_t workspace_bytes, int batch, int num_q_heads, int num_kv_heads,
+                     int head_dim, int block_size, int max_blocks, int num_pages,
+                     int max_query_len, float scale, int dtype, hipStream_t stream);
+
+/*
+ * Decode attention (as ivakv_decode_attn: q and out [batch][Hq][D], the key at context_lens[b]-1
+ * the newest, window and sinks) of a batch whose sequences share their first pages.  Group g
+ * is rows group_start[g] .. group_start[g+1]-1 (group_start [n_groups + 1], rising; rows of no group
+ * share nothing), and the block-table rows of a group agree in the full pages of its first
+ * prefix_lens[g] tokens: those are read once, from the table of the group's first row that is as
+ * long as the prefix, for all its rows; every row then walks the rest of its own pages and joins
+ * the two.  max_group: rows of
+ * the largest group at most (further rows of a group walk everything themselves, as does a row
+ * shorter than the prefix).  Two launches, no host synchronisation.  k_scale / v_scale, workspace
+ * (ivakv_prefix_workspace_size): as for ivakv_cross_attn.
+ * Replaces: the cache branch of AttentionTorch.forward (src/core/attention.py:77-102) on
+ * forked sequences.
+ */
+int ivakv_prefix_workspace_size(int batch, int n_groups, int max_group, int num_q_heads,
+                                int num_kv_heads, int head_dim, int dtype, int fp8, size_t* bytes);
+int ivakv_prefix_decode_attn(const void* q, const void* k_pool, const void* v_pool,
+                             const float* k_scale, const float* v_scale,
+                             const int32_t* block_tables, const int32_t* context_lens,
+                             const int32_t* group_start, const int32_t* prefix_lens, int n_groups,
+                             void* out, void* workspace, size_t workspace_bytes, int batch,
+                             int num_q_heads, int num_kv_heads, int head_dim, int block_size,
+                             int max_blocks, int num_pages, int max_group, float scale, int window,
+                             int n_sink, int dtype, hipStream_t stream);
+
+/*
+ * Rows of logits [n][vocab] (row_stride elements apart, each row dense): logprobs[i] = the log
+ * probability of tokens[i] (0 where the token is outside [0, vocab): padding), entropy[i] in nats,
+ * and the `top` most likely tokens in order (equal logits by index) with their log probabilities,
+ * top <= min(vocab, 64).  A logit of -inf has probability 0; a row of nothing else has log
+ * probabilities -inf and entropy 0; a NaN or +inf makes its row's results NaN (a NaN leads the
+ * order).  stats ([n][2], may be NULL): what the gradient call needs.  Sums in fp32.
+ * Replaces: log_softmax + gather over Transformer.forward's logits
+ * (src/core/transformer.py:242-255) and the top-k of generate's sampling (:292-313).
+ */
+int ivakv_token_logprobs(const void* logits, int64_t row_stride, const int64_t* tokens, int64_t n,
+                         int vocab, int top, float* logprobs, float* entropy, float* stats,
+                         float* top_logprobs, int64_t* top_tokens, int dtype, hipStream_t stream);
+/*
+ * The gradient by the logits ([n][vocab] dense, logits' dtype) of sum_i grad_logprobs[i] logprobs[i]
+ * + grad_entropy[i] entropy[i] + sum_j grad_top[i][j] top_logprobs[i][j], with that call's logits,
+ * tokens, entropy, stats and top_tokens.  Zero for rows without a finite logit.
+ */
+int ivakv_token_logprobs_grad(const void* logits, int64_t row_stride, const int64_t* tokens,
+                              const float* entropy, const float* stats, const int64_t* top_tokens,
+                              const float* grad_logprobs, const float* grad_entropy,
+                              const float* grad_top, int64_t n, int vocab, int top, void* grad,
+                              int dtype, hipStream_t stream);
+
+/*
  * Index gather on a contiguous-layout cache kv = [batch][n_heads][seq_len][D]
  * with element strides (s_b, s_h, s_s, s_d):
  *   out[b, h, j, :] = kv[b, h, indices[j], :]      out = [B][H][n_idx][D] dense

@@ -11,6 +11,7 @@ from . import _abi, model, paged_cache, workloads
 from .ops import (
     chunk_elems,
     copy_pages,
+    cross_workspace_bytes,
     decode_workspace_bytes,
     dtype_code,
     is_fp8,
@@ -19,16 +20,21 @@ from .ops import (
     kv_gather,
     kv_ops,
     KVOps,
+    paged_cross_attention,
     paged_decode_append_attention,
     paged_decode_attention,
     paged_decode_attention_merge,
     paged_decode_attention_partial,
     paged_prefill_attention,
+    paged_prefix_decode_attention,
+    prefix_workspace_bytes,
     prefill_split_workspace_bytes,
     pool_geometry,
     pool_shapes,
     rope_,
     scale_shape,
+    token_logprobs,
+    TokenLogprobs,
 )
 from .model import PagedAttention, Transformer, TransformerConfig, get_attention
 from .paged_cache import OutOfPagesError, PagedKVCache, PagedKVPool, create_kv_cache
@@ -44,6 +50,7 @@ __all__ = [
     "get_attention",
     "chunk_elems",
     "copy_pages",
+    "cross_workspace_bytes",
     "decode_workspace_bytes",
     "dtype_code",
     "is_fp8",
@@ -52,14 +59,19 @@ __all__ = [
     "kv_gather",
     "kv_ops",
     "KVOps",
+    "paged_cross_attention",
     "paged_decode_append_attention",
     "paged_decode_attention",
     "paged_decode_attention_merge",
     "paged_decode_attention_partial",
     "paged_prefill_attention",
+    "paged_prefix_decode_attention",
+    "prefix_workspace_bytes",
     "prefill_split_workspace_bytes",
     "pool_geometry",
     "pool_shapes",
     "rope_",
     "scale_shape",
+    "token_logprobs",
+    "TokenLogprobs",
 ]

@@ -180,6 +180,49 @@ SIGNATURES = {
         c_int, c_int, c_int,                   # window, n_sink, dtype
         c_void_p,                              # stream
     ]),
+    "ivakv_cross_workspace_size": (c_int, [
+        c_int, c_int, c_int, c_int,            # batch, n_tok, max_query_len, num_q_heads
+        c_int, c_int, c_int, c_int,            # num_kv_heads, head_dim, dtype, fp8
+        POINTER(c_size_t),                     # bytes
+    ]),
+    "ivakv_cross_attn": (c_int, [
+        c_void_p, c_void_p, c_void_p,          # q, k_pool, v_pool
+        c_void_p, c_void_p,                    # k_scale, v_scale
+        c_void_p, c_void_p, c_void_p,          # block_tables, context_lens, query_start
+        c_int, c_void_p,                       # n_tok, out
+        c_void_p, c_size_t,                    # workspace, workspace_bytes
+        c_int, c_int, c_int, c_int,            # batch, num_q_heads, num_kv_heads, head_dim
+        c_int, c_int, c_int, c_int, c_float,   # block_size, max_blocks, num_pages, max_query_len, scale
+        c_int, c_void_p,                       # dtype, stream
+    ]),
+    "ivakv_prefix_workspace_size": (c_int, [
+        c_int, c_int, c_int, c_int,            # batch, n_groups, max_group, num_q_heads
+        c_int, c_int, c_int, c_int,            # num_kv_heads, head_dim, dtype, fp8
+        POINTER(c_size_t),                     # bytes
+    ]),
+    "ivakv_prefix_decode_attn": (c_int, [
+        c_void_p, c_void_p, c_void_p,          # q, k_pool, v_pool
+        c_void_p, c_void_p,                    # k_scale, v_scale
+        c_void_p, c_void_p,                    # block_tables, context_lens
+        c_void_p, c_void_p, c_int,             # group_start, prefix_lens, n_groups
+        c_void_p, c_void_p, c_size_t,          # out, workspace, workspace_bytes
+        c_int, c_int, c_int, c_int,            # batch, num_q_heads, num_kv_heads, head_dim
+        c_int, c_int, c_int, c_int, c_float,   # block_size, max_blocks, num_pages, max_group, scale
+        c_int, c_int, c_int, c_void_p,         # window, n_sink, dtype, stream
+    ]),
+    "ivakv_token_logprobs": (c_int, [
+        c_void_p, c_int64, c_void_p, c_int64,  # logits, row_stride, tokens, n
+        c_int, c_int, c_void_p, c_void_p,      # vocab, top, logprobs, entropy
+        c_void_p, c_void_p, c_void_p,          # stats, top_logprobs, top_tokens
+        c_int, c_void_p,                       # dtype, stream
+    ]),
+    "ivakv_token_logprobs_grad": (c_int, [
+        c_void_p, c_int64, c_void_p,           # logits, row_stride, tokens
+        c_void_p, c_void_p, c_void_p,          # entropy, stats, top_tokens
+        c_void_p, c_void_p, c_void_p,          # grad_logprobs, grad_entropy, grad_top
+        c_int64, c_int, c_int, c_void_p,       # n, vocab, top, grad
+        c_int, c_void_p,                       # dtype, stream
+    ]),
     "ivakv_chunk_slots": (c_int, [
         c_void_p, c_void_p, c_int, c_int,      # block_tables, context_lens, batch, n
         c_int, c_int, c_void_p, c_void_p,      # max_blocks, block_size, slots, stream

@@ -16,7 +16,7 @@ from __future__ import annotations
 import ctypes
 import math
 from functools import lru_cache, partial
-from typing import Dict, List, Optional, Tuple
+from typing import Dict, List, NamedTuple, Optional, Tuple
 
 import torch
 
@@ -698,6 +698,262 @@ def paged_prefill_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
               num_pages, int(max_query_len), float(scale), window, n_sink, dtype_code(q.dtype),
               _stream(dev))
     return out
+
+
+def _row_attention(q, k_pool, v_pool, block_tables, context_lens, starts, k_scale, v_scale, out):
+    """The checks that cross attention and shared-prefix attention share: (device, pool geometry,
+    FP8 factors or (None, None), int32 operands, contiguous q, out)."""
+    dev = _require_gpu(q, k_pool, v_pool, block_tables, context_lens, starts)
+    geometry = pool_geometry(k_pool, v_pool)
+    head_dim = geometry[2]
+    if q.dim() != 3 or q.shape[2] != head_dim:
+        raise ValueError(f"q must be [rows, Hq, {head_dim}]; got {tuple(q.shape)}")
+    scales = (None, None)
+    if is_fp8(k_pool):
+        if q.dtype not in (torch.float16, torch.bfloat16):
+            raise TypeError(f"FP8 pools take float16 or bfloat16 queries, got {q.dtype}")
+        scales = tuple(t.data_ptr() for t in _scales(k_pool, k_scale, v_scale))
+    elif q.dtype != k_pool.dtype:
+        raise TypeError(f"q dtype {q.dtype} != pool dtype {k_pool.dtype}")
+    block_tables = _i32(block_tables, "block_tables")
+    context_lens = _i32_row(context_lens, "context_lens")
+    if block_tables.dim() != 2 or block_tables.shape[0] != context_lens.numel():
+        raise ValueError("block_tables must be [B, max_blocks] with B == len(context_lens)")
+    q = q.contiguous()
+    if out is None:
+        out = torch.empty_like(q)
+    else:
+        if out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+            raise ValueError("out must be a contiguous tensor shaped and typed like q")
+        _buffer(out, dev, "out")
+    return dev, geometry, scales, block_tables, context_lens, q, out
+
+
+def _longest_run(starts: torch.Tensor, n: int, name: str, last_is_n: bool, missing: str,
+                 dev: torch.device) -> int:
+    """The largest step of a row of starts, read back from the device and checked."""
+    if _capturing(dev):
+        raise ValueError(f"{missing} is required under HIP-graph capture (the host cannot read "
+                         f"{name} then)")
+    s = starts.tolist()
+    if s[0] < 0 or s[-1] > n or any(b < a for a, b in zip(s, s[1:])) or \
+            (last_is_n and (s[0] != 0 or s[-1] != n)):
+        bounds = f"from 0 to {n}" if last_is_n else f"within [0, {n}]"
+        raise ValueError(f"{name} must rise {bounds}; got "
+                         f"{s if len(s) <= 8 else s[:4] + ['...'] + s[-4:]}")
+    return max((b - a for a, b in zip(s, s[1:])), default=0)
+
+
+def _sized_workspace(workspace, dev: torch.device, nbytes: int) -> torch.Tensor:
+    """The caller's workspace, checked, or the op's own: that of the device and stream, or under
+    HIP-graph capture one of the graph's own memory, so that graphs captured on one stream may
+    be replayed on several."""
+    if workspace is None:
+        if _capturing(dev):
+            return torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
+        return _workspace(dev, nbytes)
+    if workspace.numel() * workspace.element_size() < nbytes:
+        raise ValueError(f"workspace has {workspace.numel() * workspace.element_size()} bytes, "
+                         f"{nbytes} needed")
+    return _buffer(workspace, dev, "workspace")
+
+
+@lru_cache(maxsize=1024)
+def _row_workspace_bytes(entry: str, *geometry: int) -> int:
+    out = ctypes.c_size_t(0)
+    _abi.call(entry, *geometry, ctypes.byref(out))
+    return int(out.value)
+
+
+def cross_workspace_bytes(batch: int, n_tok: int, max_query_len: int, num_q_heads: int,
+                          num_kv_heads: int, head_dim: int, dtype: torch.dtype,
+                          fp8: bool = False) -> int:
+    """Workspace bytes of :func:`paged_cross_attention` (``dtype`` of the queries, ``fp8``: FP8
+    pools).  The workspace needs no initialisation."""
+    return _row_workspace_bytes("ivakv_cross_workspace_size", int(batch), int(n_tok),
+                                int(max_query_len), int(num_q_heads), int(num_kv_heads),
+                                int(head_dim), dtype_code(dtype), int(fp8))
+
+
+def paged_cross_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                          block_tables: torch.Tensor, context_lens: torch.Tensor,
+                          query_start: torch.Tensor, scale: Optional[float] = None,
+                          max_query_len: Optional[int] = None,
+                          out: Optional[torch.Tensor] = None,
+                          k_scale: Optional[torch.Tensor] = None,
+                          v_scale: Optional[torch.Tensor] = None,
+                          workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Cross attention: a decoder's rows over states of another length kept in pages.
+
+    ``q`` is ``[n_tok, Hq, D]``; the rows of sequence b are ``query_start[b] ..
+    query_start[b+1]-1`` (int32 ``[B+1]``) and attend to all of its ``context_lens[b]`` keys, with no
+    causal mask (one row per sequence: a single-token step).  A row without keys gives zeros.
+    ``max_query_len`` (>= every sequence's rows) sizes the launch; when omitted it is read back from
+    ``query_start`` (a device sync), which is then checked.  Pools, FP8 factors and ``scale`` as in
+    :func:`paged_prefill_attention`; ``workspace`` (:func:`cross_workspace_bytes`) is kept per
+    device and stream when omitted.  Returns ``[n_tok, Hq, D]``.
+
+    Replaces ``AttentionTorch.forward`` with ``config.causal`` False (src/core/attention.py:77-102).
+    """
+    dev, (num_pages, hkv, head_dim, bs), scales, block_tables, context_lens, q, out = _row_attention(
+        q, k_pool, v_pool, block_tables, context_lens, query_start, k_scale, v_scale, out)
+    n_tok, hq, _ = q.shape
+    query_start = _i32_row(query_start, "query_start")
+    batch = context_lens.numel()
+    if query_start.numel() != batch + 1:
+        raise ValueError(f"query_start must have B+1 = {batch + 1} entries")
+    if max_query_len is None:
+        max_query_len = _longest_run(query_start, n_tok, "query_start", True, "max_query_len", dev)
+    if scale is None:
+        scale = 1.0 / math.sqrt(head_dim)
+    workspace = _sized_workspace(workspace, dev, cross_workspace_bytes(
+        batch, n_tok, max_query_len, hq, hkv, head_dim, q.dtype, scales[0] is not None))
+    _abi.call("ivakv_cross_attn", q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), *scales,
+              block_tables.data_ptr(), context_lens.data_ptr(), query_start.data_ptr(), n_tok,
+              out.data_ptr(), workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+              batch, hq, hkv, head_dim, bs, block_tables.shape[1], num_pages, int(max_query_len),
+              float(scale), dtype_code(q.dtype), _stream(dev))
+    return out
+
+
+def prefix_workspace_bytes(batch: int, n_groups: int, max_group: int, num_q_heads: int,
+                           num_kv_heads: int, head_dim: int, dtype: torch.dtype,
+                           fp8: bool = False) -> int:
+    """Workspace bytes of :func:`paged_prefix_decode_attention` (``dtype`` of the queries,
+    ``fp8``: FP8 pools).  The workspace needs no initialisation."""
+    return _row_workspace_bytes("ivakv_prefix_workspace_size", int(batch), int(n_groups),
+                                int(max_group), int(num_q_heads), int(num_kv_heads),
+                                int(head_dim), dtype_code(dtype), int(fp8))
+
+
+def paged_prefix_decode_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                                  block_tables: torch.Tensor, context_lens: torch.Tensor,
+                                  group_start: torch.Tensor, prefix_lens: torch.Tensor,
+                                  scale: Optional[float] = None, window: Optional[int] = None,
+                                  n_sink: int = 0, max_group: Optional[int] = None,
+                                  out: Optional[torch.Tensor] = None,
+                                  workspace: Optional[torch.Tensor] = None,
+                                  k_scale: Optional[torch.Tensor] = None,
+                                  v_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """:func:`paged_decode_attention` of a batch whose sequences share their first pages
+    (``PagedKVPool.fork``): the shared pages are read once for all of a group's rows.
+
+    Rows ``group_start[g] .. group_start[g+1]-1`` (int32 ``[n_groups+1]``, rising) form group g, and
+    their block-table rows have to agree in the full pages of the group's first ``prefix_lens[g]``
+    tokens (int32 ``[n_groups]``); those are read from the table of the first row that is as long.
+    Rows of no group, and rows shorter than their group's prefix, read all of their own pages.  Same result as
+    :func:`paged_decode_attention` within the attention tolerance.  ``max_group`` (>= the largest
+    group's rows) sizes the launch; when omitted it is read back from ``group_start`` (a device
+    sync), which is then checked.  ``workspace`` (:func:`prefix_workspace_bytes`) is kept per device
+    and stream when omitted.
+
+    Replaces the cache branch of ``AttentionTorch.forward`` (src/core/attention.py:77-102).
+    """
+    dev, (num_pages, hkv, head_dim, bs), scales, block_tables, context_lens, q, out = _row_attention(
+        q, k_pool, v_pool, block_tables, context_lens, group_start, k_scale, v_scale, out)
+    batch, hq, _ = q.shape
+    if context_lens.numel() != batch:
+        raise ValueError(f"context_lens has {context_lens.numel()} entries for {batch} rows")
+    group_start = _i32_row(group_start, "group_start")
+    prefix_lens = _i32_row(prefix_lens, "prefix_lens")
+    _require_gpu(q, prefix_lens)
+    n_groups = prefix_lens.numel()
+    if group_start.numel() != n_groups + 1:
+        raise ValueError(f"group_start must have n_groups+1 = {n_groups + 1} entries")
+    if max_group is None:
+        max_group = _longest_run(group_start, batch, "group_start", False, "max_group", dev)
+    if scale is None:
+        scale = 1.0 / math.sqrt(head_dim)
+    workspace = _sized_workspace(workspace, dev, prefix_workspace_bytes(
+        batch, n_groups, max_group, hq, hkv, head_dim, q.dtype, scales[0] is not None))
+    _abi.call("ivakv_prefix_decode_attn", q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), *scales,
+              block_tables.data_ptr(), context_lens.data_ptr(), group_start.data_ptr(),
+              prefix_lens.data_ptr(), n_groups, out.data_ptr(), workspace.data_ptr(),
+              workspace.numel() * workspace.element_size(), batch, hq, hkv, head_dim, bs,
+              block_tables.shape[1], num_pages, int(max_group), float(scale),
+              int(window) if window else 0, int(n_sink) if n_sink else 0, dtype_code(q.dtype),
+              _stream(dev))
+    return out
+
+
+MAX_TOP_LOGPROBS = 64
+
+
+class TokenLogprobs(NamedTuple):
+    """What :func:`token_logprobs` returns; the leading dims are those of the logits."""
+    logprobs: torch.Tensor       # float32 [...]
+    entropy: torch.Tensor        # float32 [...], nats
+    top_logprobs: torch.Tensor   # float32 [..., top_k]
+    top_tokens: torch.Tensor     # int64 [..., top_k]
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits: torch.Tensor, tokens: torch.Tensor, top_k: int, keep: bool):
+        n, vocab = logits.shape
+        dev = logits.device
+        logprobs = torch.empty(n, dtype=torch.float32, device=dev)
+        entropy = torch.empty(n, dtype=torch.float32, device=dev)
+        stats = torch.empty(n, 2, dtype=torch.float32, device=dev) if keep else None
+        top = torch.empty(n, top_k, dtype=torch.float32, device=dev)
+        top_tokens = torch.empty(n, top_k, dtype=torch.int64, device=dev)
+        _abi.call("ivakv_token_logprobs", logits.data_ptr(), logits.stride(0), tokens.data_ptr(), n,
+                  vocab, top_k, logprobs.data_ptr(), entropy.data_ptr(),
+                  stats.data_ptr() if keep else None, top.data_ptr(), top_tokens.data_ptr(),
+                  dtype_code(logits.dtype), _stream(dev))
+        if keep:
+            ctx.save_for_backward(logits, tokens, entropy, stats, top_tokens)
+        ctx.mark_non_differentiable(top_tokens)
+        return logprobs, entropy, top, top_tokens
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g, gh, gt, _):
+        logits, tokens, entropy, stats, top_tokens = ctx.saved_tensors
+        n, vocab = logits.shape
+        grad = torch.empty(n, vocab, dtype=logits.dtype, device=logits.device)
+        g, gh, gt = (t.contiguous() for t in (g, gh, gt))
+        _abi.call("ivakv_token_logprobs_grad", logits.data_ptr(), logits.stride(0),
+                  tokens.data_ptr(), entropy.data_ptr(), stats.data_ptr(), top_tokens.data_ptr(),
+                  g.data_ptr(), gh.data_ptr(), gt.data_ptr(), n, vocab, top_tokens.shape[1],
+                  grad.data_ptr(), dtype_code(logits.dtype), _stream(logits.device))
+        return grad, None, None, None
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0) -> TokenLogprobs:
+    """Log probabilities of given tokens under rows of logits, with each row's entropy and its
+    ``top_k`` most likely tokens, in one pass over the logits.
+
+    ``logits`` is ``[..., V]`` (float32, float16 or bfloat16), ``tokens`` integers of the leading
+    shape.  A token outside ``[0, V)`` (padding, say -100) has log probability 0 and no gradient.
+    ``top_k`` <= min(V, 64); equal logits go by index.  A logit of -inf has probability 0; a row of
+    nothing else has log probabilities -inf, entropy 0 and gradient 0; NaN or +inf in a row makes
+    its results NaN.  Differentiable by the logits through ``logprobs``, ``entropy`` and
+    ``top_logprobs`` (once).
+
+    Replaces ``log_softmax`` and a gather over ``Transformer.forward``'s logits
+    (src/core/transformer.py:242-255).
+    """
+    dev = _require_gpu(logits, tokens)
+    dtype_code(logits.dtype)  # (raises for other types)
+    if logits.dim() < 1 or tuple(tokens.shape) != tuple(logits.shape[:-1]):
+        raise ValueError(f"tokens must be shaped like the logits' leading dims {tuple(logits.shape[:-1])}; "
+                         f"got {tuple(tokens.shape)}")
+    if tokens.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"tokens must be int64 or int32, got {tokens.dtype}")
+    vocab, top_k = logits.shape[-1], int(top_k)
+    if not 0 <= top_k <= min(vocab, MAX_TOP_LOGPROBS):
+        raise ValueError(f"top_k must be in [0, {min(vocab, MAX_TOP_LOGPROBS)}], got {top_k}")
+    lead = tuple(tokens.shape)
+    rows = logits.reshape(-1, vocab) if vocab else logits.reshape(tokens.numel(), 0)
+    if rows.shape[0] and not vocab:
+        raise ValueError("rows without logits")
+    if rows.numel() and rows.stride(1) != 1:
+        rows = rows.contiguous()
+    flat = tokens.reshape(-1).to(torch.int64).contiguous()
+    keep = torch.is_grad_enabled() and logits.requires_grad
+    lp, h, top, ids = _TokenLogprobs.apply(rows, flat, top_k, keep)
+    return TokenLogprobs(lp.view(lead), h.view(lead), top.view(*lead, top_k), ids.view(*lead, top_k))
 
 
 def rope_(x: torch.Tensor, positions: torch.Tensor, theta: float = 10000.0) -> torch.Tensor:

@@ -439,3 +439,40 @@ def index_scatter(kv: np.ndarray, indices: np.ndarray, values: np.ndarray) -> np
     out = kv.copy()
     out[:, :, np.asarray(indices, dtype=np.int64), :] = values
     return out
+
+
+def cross_attention(q: np.ndarray, k_pool: np.ndarray, v_pool: np.ndarray, block_tables: np.ndarray,
+                    ctx_lens: np.ndarray, query_start: np.ndarray,
+                    scale: Optional[float] = None) -> np.ndarray:
+    """fp64 attention of every row of ``q`` ([n_tok, Hq, D], rows of sequence b at
+    ``query_start[b] ..``) over all keys of its sequence: :func:`decode_attention` of each row
+    with its sequence's table."""
+    qs = np.asarray(query_start, dtype=np.int64)
+    seq = np.repeat(np.arange(len(qs) - 1), np.diff(qs))
+    return decode_attention(q, k_pool, v_pool, np.asarray(block_tables)[seq],
+                            np.asarray(ctx_lens)[seq], scale=scale)
+
+
+def token_logprobs(logits: np.ndarray, tokens: np.ndarray, top_k: int = 0):
+    """fp64 (log probabilities of ``tokens`` [n], entropy [n], the top_k log probabilities and
+    tokens [n, top_k]) of rows of logits [n, V]: log_softmax, -sum p log p with 0 log 0 = 0, a stable
+    descending sort (equal logits by index).  A token outside [0, V) has log probability 0; a row
+    without a finite logit has log probabilities -inf and entropy 0; NaN or +inf makes the row NaN."""
+    z = np.asarray(logits, dtype=np.float64)
+    n, v = z.shape
+    top = z.max(axis=1, keepdims=True)
+    none = np.isneginf(top)
+    with np.errstate(invalid="ignore", divide="ignore"):
+        d = z - np.where(none, 0.0, top)
+        e = np.exp(d)
+        logp = d - np.log(np.where(none, 1.0, e.sum(axis=1, keepdims=True)))
+        p = np.exp(logp)
+        entropy = -np.where(p == 0, 0.0, p * logp).sum(axis=1)
+    t = np.asarray(tokens)
+    given = (t >= 0) & (t < v)
+    picked = np.where(given, logp[np.arange(n), np.where(given, t, 0)], 0.0)
+    # NaN first, then by value, equal values in index order
+    order = np.lexsort((np.broadcast_to(np.arange(v), z.shape), -np.nan_to_num(z, nan=0.0, posinf=np.inf,
+                                                                              neginf=-np.inf), ~np.isnan(z)),
+                       axis=1)[:, :top_k]
+    return picked, entropy, np.take_along_axis(logp, order, axis=1), order
