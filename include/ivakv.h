@@ -433,12 +433,13 @@ int ivakv_prefill_attn_split_fp8(const void* q, const void* k_pool, const void* 
  * in ivakv_prefill_attn (rows of a sequence past max_query_len, and rows of no sequence, are
  * left as they are); a row without keys gives zeros.  k_scale / v_scale: the factors of FP8
  * pools (fp16 or bf16 queries), NULL for pools of the queries' type.  Two launches at most, no
- * host synchronisation.  The workspace (ivakv_cross_workspace_size; fp8: 1 for FP8 pools) needs no
- * initialisation; calls that share one must not run concurrently.
+ * host synchronisation.  The workspace (ivakv_cross_workspace_size) needs no initialisation;
+ * calls that share one must not run concurrently.
  * Replaces: AttentionTorch.forward with config.causal False (src/core/attention.py:77-102).
  */
 int ivakv_cross_workspace_size(int batch, int n_tok, int max_query_len, int num_q_heads,
-                               int num_kv_heads, int head_dim, int dtype, int fp8, size_t* bytes);
+                               int num_kv_heads, int head_dim, int max_blocks, int dtype,
+                               size_t* bytes);
 int ivakv_cross_attn(const void* q, const void* k_pool, const void* v_pool, const float* k_scale,
                      const float* v_scale, const int32_t* block_tables, const int32_t* context_lens,
                      const int32_t* query_start, int n_tok, void* out, void* workspace,
@@ -451,17 +452,19 @@ int ivakv_cross_attn(const void* q, const void* k_pool, const void* v_pool, cons
  * the newest, window and sinks) of a batch whose sequences share their first pages.  Group g
  * is rows group_start[g] .. group_start[g+1]-1 (group_start [n_groups + 1], rising; rows of no group
  * share nothing), and the block-table rows of a group agree in the full pages of its first
- * prefix_lens[g] tokens: those are read once, from the table of the group's first row that is as
- * long as the prefix, for all its rows; every row then walks the rest of its own pages and joins
- * the two.  max_group: rows of
- * the largest group at most (further rows of a group walk everything themselves, as does a row
- * shorter than the prefix).  Two launches, no host synchronisation.  k_scale / v_scale, workspace
- * (ivakv_prefix_workspace_size): as for ivakv_cross_attn.
+ * prefix_lens[g] tokens: those are read once, from the table of the group's first row that takes
+ * part, for all its rows; every row walks the rest of its own pages, and a second launch joins the
+ * two.  A row takes part if it has the whole prefix and its window cuts nothing off; any other walks
+ * all of its visible pages itself, as do rows past max_group of a group (max_group: rows of the
+ * largest group).  batch <= 8192, batch x max_blocks x num_kv_heads < 2^31.  No host
+ * synchronisation.  k_scale / v_scale, workspace (ivakv_prefix_workspace_size): as for
+ * ivakv_cross_attn.
  * Replaces: the cache branch of AttentionTorch.forward (src/core/attention.py:77-102) on
  * forked sequences.
  */
 int ivakv_prefix_workspace_size(int batch, int n_groups, int max_group, int num_q_heads,
-                                int num_kv_heads, int head_dim, int dtype, int fp8, size_t* bytes);
+                                int num_kv_heads, int head_dim, int max_blocks, int dtype,
+                                size_t* bytes);
 int ivakv_prefix_decode_attn(const void* q, const void* k_pool, const void* v_pool,
                              const float* k_scale, const float* v_scale,
                              const int32_t* block_tables, const int32_t* context_lens,

@@ -182,7 +182,7 @@ SIGNATURES = {
     ]),
     "ivakv_cross_workspace_size": (c_int, [
         c_int, c_int, c_int, c_int,            # batch, n_tok, max_query_len, num_q_heads
-        c_int, c_int, c_int, c_int,            # num_kv_heads, head_dim, dtype, fp8
+        c_int, c_int, c_int, c_int,            # num_kv_heads, head_dim, max_blocks, dtype
         POINTER(c_size_t),                     # bytes
     ]),
     "ivakv_cross_attn": (c_int, [
@@ -197,7 +197,7 @@ SIGNATURES = {
     ]),
     "ivakv_prefix_workspace_size": (c_int, [
         c_int, c_int, c_int, c_int,            # batch, n_groups, max_group, num_q_heads
-        c_int, c_int, c_int, c_int,            # num_kv_heads, head_dim, dtype, fp8
+        c_int, c_int, c_int, c_int,            # num_kv_heads, head_dim, max_blocks, dtype
         POINTER(c_size_t),                     # bytes
     ]),
     "ivakv_prefix_decode_attn": (c_int, [

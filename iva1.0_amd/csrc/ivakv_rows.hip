@@ -15,14 +15,15 @@
 // both pages) are the PV product's B operand, so nothing passes through LDS but the end of
 // the walk.  The softmax runs online in fp32 in the log2 domain.
 //
-// Split: a workgroup of four waves takes a chunk of 16 NR rows and a segment of the unit's pages,
-// wave w the page pairs w, w + 4, ...; the four states meet in LDS and leave one partial (running
-// max, sum, unnormalized rows).  Segments are sized on the device from the groups' pages, so that
-// ragged groups fill the CUs evenly; a second launch joins a row's partials.  For the prefix that
-// launch walks each sequence's own pages first (prefix_own_kernel).
+// Split: a workgroup takes a chunk of 16 NR rows and a segment of the unit's pages, its waves the page
+// pairs in turn; their states meet in LDS and leave one partial (running max, sum, unnormalized
+// rows).  Segments are sized on the device from the groups' pages, so that ragged groups fill the
+// CUs evenly.  The prefix op's own pages are walked in the same launch by workgroups behind those:
+// waves with equal shares of all (sequence, kv head, page pair) tiles, as the decode walk has them.  A
+// second launch joins a row's partials.
 //
-// Bound: the K and V bytes of the shared pages, read once for up to 16 NR rows; from a few
-// hundred rows on the matrix and vector pipes (4 D operations per key and row).
+// Bound: the K and V bytes of the shared pages, read once for up to 16 NR rows, and of the own
+// pages; from a few hundred rows on the matrix and vector pipes (4 D operations per key and row).
 #include <type_traits>
 
 #include "ivakv_tile.h"
@@ -32,8 +33,6 @@ namespace {
 
 // Log2-domain headroom of the lazy row max, as in the prefill: p = exp2(s - m) stays <= 2^8.
 constexpr float kLazyMax = 8.f;
-constexpr int kWaves = 4;
-constexpr int kThreads = 64 * kWaves;
 
 struct RowArgs {
   const void* q;  // [n_rows, Hq, D]
@@ -46,13 +45,18 @@ struct RowArgs {
   const int32_t* ctx;    // cross: keys of each group; prefix: length of each row's sequence
   const int32_t* start;  // [n_groups + 1] first query row of each group
   const int32_t* shared; // prefix: [n_groups] shared tokens
-  float* part_acc;       // [slot][16 NR][D]
+  float* part_acc;       // shared partials [slot][16 NR][D]
   float* part_ml;        // [slot][16 NR][2]  (running max, sum)
+  float* own_acc;        // own partials [slot][G][D]
+  float* own_ml;         // [slot][G][2]
+  int32_t* own_pref;     // [n_rows + 1] own page sets before each row
   int n_groups, n_rows, Hkv, G, max_blocks, num_pages;
   int prefix;            // 1: prefix groups, 0: cross
   int max_rows;          // query rows of the largest group
-  int chunks, rows_chunk;  // its row chunks, rows of a chunk (16 NR)
-  int segments;          // segments of all groups the grid holds
+  int rows_shift;        // log2 of the rows of a chunk (16 NR)
+  int items, split;      // (piece, row chunk) pairs the grid holds for a kv head; whether pages are cut
+  int unit;              // pages a shared workgroup's waves take at once
+  int shared_wgs, own_waves;  // workgroups of the shared walk, waves of the own walk
   float scale_log2;
   int window, n_sink;
 };
@@ -199,12 +203,9 @@ struct PageOps<DT, D, true> {
 struct KeyList {
   const int32_t* row;  // block-table row
   int num_pages;
-  // Logical page of list entry v: three runs of consecutive pages.
-  int a0, na, b0, nb, c0;
+  int na, c0;          // list entry v: logical page v below na, then c0 + v - na
   int len, win_start, n_sink;  // keys < len, and >= win_start or < n_sink
-  IVAKV_INLINE __device__ inline int page(int v) const {
-    return v < na ? a0 + v : v < na + nb ? b0 + (v - na) : c0 + (v - na - nb);
-  }
+  IVAKV_INLINE __device__ inline int page(int v) const { return v < na ? v : c0 + (v - na); }
   IVAKV_INLINE __device__ inline bool full(int lp) const {
     return lp * kBS + kBS <= len && (lp * kBS >= win_start || lp * kBS + kBS <= n_sink);
   }
@@ -217,8 +218,8 @@ struct KeyList {
   }
 };
 
-// The online softmax of NR blocks of 16 rows and its walk over a list of pages.
-template <int DT, int D, bool kFp8, int NR>
+// kRegs: the registers of a lane that the kernel's occupancy leaves it.
+template <int DT, int D, bool kFp8, int NR, int kRegs>
 struct Walk {
   using Ops = PageOps<DT, D, kFp8>;
   using Tr = typename Ops::Tr;
@@ -228,38 +229,59 @@ struct Walk {
   // product with ones, so the rounding of P (2^-9 relative in bf16, 2^-12 in fp16) cancels
   // where one key dominates.  FP8 and fp32 sum the weights in fp32.
   static constexpr bool kSumMfma = !kFp8 && DT != IVAKV_F32;
-  typename Ops::QReg q[NR];
+  // With many row blocks, or long rows, the rows' operands stay in LDS, in lane order (one copy per workgroup), and
+  // leave their registers to the accumulators.
+  static constexpr bool kQLds = NR >= 4 || (NR >= 2 && D * sizeof(E) >= 512);
+  static constexpr int kQBytes = kQLds ? 16 * NR * D * (int)sizeof(E) : 0;
+  typename Ops::QReg q[kQLds ? 1 : NR];
+  const Chunk16* q_lds;
   f32x4 acc[NR][NB];
   f32x4 lacc[kSumMfma ? NR : 1];
   float m[NR], l[NR], grow_at[NR], neg_m[NR];
   float c, inv_c;  // |scale| log2(e)
 
-  IVAKV_INLINE __device__ inline void init(const RowArgs& a, int64_t row0, int n, int h,
-                                                            int r0, int ln, int lq) {
+  // Rows r0 .. r0 + 16 NR - 1 of n (row r: query row row0 + r / G, head r % G of kv head h).  Every
+  // wave of the workgroup calls it; with kQLds it ends in a barrier.
+  template <int W>
+  IVAKV_INLINE __device__ inline void init(const RowArgs& a, int64_t row0, int n, int h, int r0, int wave,
+                                           int ln, int lq, Chunk16* lds) {
     c = fmaxf(fabsf(a.scale_log2), 1.17549435e-38f);
     inv_c = 1.f / c;
+    q_lds = lds + 16 * lq + ln;
     const int Hq = a.Hkv * a.G;
-#pragma unroll
-    for (int rb = 0; rb < NR; ++rb) {
+    // a negative scale negates q instead (exact)
+    const uint32_t sign = a.scale_log2 >= 0.f ? 0u : sizeof(E) == 2 ? 0x80008000u : 0x80000000u;
+    auto chunk = [&](int rb, int j) IVAKV_INLINE -> Chunk16 {
       const int r = min(r0 + 16 * rb + ln, n - 1);  // rows past the end repeat the last one
       const E* p = static_cast<const E*>(a.q) + ((row0 + r / a.G) * Hq + h * a.G + r % a.G) * D;
+      Chunk16 x = *reinterpret_cast<const Chunk16*>(p + Ops::q_at(j, lq));
 #pragma unroll
-      for (int j = 0; j < Ops::NQ; ++j) q[rb].c[j] = *reinterpret_cast<const Chunk16*>(p + Ops::q_at(j, lq));
+      for (int i = 0; i < 4; ++i) x.w[i] ^= sign;
+      return x;
+    };
+    if constexpr (kQLds) {
+      for (int rb = wave; rb < NR; rb += W)
+#pragma unroll
+        for (int j = 0; j < Ops::NQ; ++j) lds[(rb * Ops::NQ + j) * 64 + 16 * lq + ln] = chunk(rb, j);
+    } else {
+#pragma unroll
+      for (int rb = 0; rb < NR; ++rb)
+#pragma unroll
+        for (int j = 0; j < Ops::NQ; ++j) q[rb].c[j] = chunk(rb, j);
+    }
+#pragma unroll
+    for (int rb = 0; rb < NR; ++rb) {
       m[rb] = grow_at[rb] = kNegInf;
       l[rb] = neg_m[rb] = 0.f;
       if constexpr (kSumMfma) lacc[rb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int b = 0; b < NB; ++b) acc[rb][b] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    if (a.scale_log2 < 0.f) {  // a negative scale negates q instead (exact)
-      const uint32_t sign = sizeof(E) == 2 ? 0x80008000u : 0x80000000u;
-#pragma unroll
-      for (int rb = 0; rb < NR; ++rb)
-#pragma unroll
-        for (int j = 0; j < Ops::NQ; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) q[rb].c[j].w[i] ^= sign;
-    }
+    if constexpr (kQLds) __syncthreads();
+  }
+  IVAKV_INLINE __device__ inline Chunk16 row(int rb, int j) const {
+    if constexpr (kQLds) return q_lds[(rb * Ops::NQ + j) * 64];
+    else return q[rb].c[j];
   }
 
   using Scores = f32x4[NR][PG];
@@ -273,7 +295,7 @@ struct Walk {
       for (int j = 0; j < Ops::NQ; ++j) {
         const Chunk16 k = Ops::key(t, i, j);
 #pragma unroll
-        for (int rb = 0; rb < NR; ++rb) s[rb][i] = Tr::qk(k, q[rb].c[j], s[rb][i]);
+        for (int rb = 0; rb < NR; ++rb) s[rb][i] = Tr::qk(k, row(rb, j), s[rb][i]);
       }
       if constexpr (kFp8) {
 #pragma unroll
@@ -336,10 +358,13 @@ struct Walk {
         mx = fmaxf(mx, __shfl_xor(mx, 32));
         const float m_new = fmaxf(m[rb], mx);
         const float f = m_new == kNegInf ? 1.f : exp2_fast(m[rb] - m_new);
-        l[rb] *= f;
-        if constexpr (kSumMfma) lacc[rb] *= f;
+        // (the first keys of a walk find sums of zero: nothing to scale)
+        if (__builtin_amdgcn_ballot_w64(m[rb] != kNegInf) != 0) {
+          l[rb] *= f;
+          if constexpr (kSumMfma) lacc[rb] *= f;
 #pragma unroll
-        for (int b = 0; b < NB; ++b) acc[rb][b] *= f;
+          for (int b = 0; b < NB; ++b) acc[rb][b] *= f;
+        }
         m[rb] = m_new;
         grow_at[rb] = (m_new + kLazyMax) * inv_c;
         neg_m[rb] = m_new == kNegInf ? 0.f : -m_new;
@@ -418,8 +443,8 @@ struct Walk {
   // blocks; K of the set after next is loaded as soon as this set's scores are there, V as soon as
   // its rows are.
   static constexpr int kSetRegs = 2 * (int)sizeof(typename Ops::Set) / 4;
-  static constexpr int kRowRegs = NR * (4 * NB + 4 * Ops::NQ + 4 * PG + 8);
-  static constexpr int kSets = kSetRegs + kRowRegs <= 320 ? 2 : 1;
+  static constexpr int kRowRegs = NR * (4 * NB + (kQLds ? 0 : 4 * Ops::NQ) + 4 * PG + 8);
+  static constexpr int kSets = kSetRegs + kRowRegs <= (kRegs > 256 ? 300 : 180) ? 2 : 1;
 
   // Walks list entries [v0, v1) PG at a time: this wave the sets w, w + W, ...  Loads past the end
   // repeat the last entry and are not folded.
@@ -531,209 +556,201 @@ __device__ inline void join_waves(const WalkT& wk, float* smem, int wave, int ln
   __syncthreads();
 }
 
-// Full pages of the first tokens of group g that its sequences share, inside the table.
-__device__ inline int shared_blocks(const RowArgs& a, int g) {
-  const int p = a.shared[g] / kBS;
-  return p < 0 ? 0 : p < a.max_blocks ? p : a.max_blocks;
-}
-
 // Rows [r0, r1) of group g, inside [0, n_rows].
 __device__ inline void group_rows(const RowArgs& a, int g, int& r0, int& r1) {
   r0 = min(max(a.start[g], 0), a.n_rows);
   r1 = min(max(a.start[g + 1], r0), a.n_rows);
 }
 
-// The part of a prefix group's shared pages that is walked for all rows.  Without a window
-// all of them.  With one, every row that has the whole prefix (length >= 16 blocks) sees the full
-// sink pages, [0, sinks), and what its own window, length - window on, leaves: the pages from
-// lo on lie in every row's window.  [base, lo) and the rest belong to the rows' own walks, as does
-// everything of a row shorter than the prefix.
-struct SharedPages {
-  int blocks, sinks, base, lo;
-  __device__ inline int listed() const { return sinks + blocks - base; }
+// One group as a lane holds it: its rows, their chunks and its pages.  prefix: the full pages of the
+// shared tokens, inside the table.  A group without rows has no chunks.
+struct Group {
+  int r0, r1, chunks, pages;
 };
-
-__device__ inline SharedPages shared_pages(const RowArgs& a, int g) {
-  SharedPages s;
-  s.blocks = shared_blocks(a, g);
-  s.sinks = s.base = 0;
-  if (a.window > 0) {
-    s.base = max(0, s.blocks - cdiv(a.window, kBS));
-    s.sinks = min(a.n_sink / kBS, s.base);
-  }
-  s.lo = s.base;
-  return s;
+__device__ inline Group load_group(const RowArgs& a, int g) {
+  Group x{0, 0, 0, 0};
+  if (g >= a.n_groups) return x;
+  const int n = a.prefix ? a.shared[g] / kBS : cdiv(max(a.ctx[g], 0), kBS);
+  group_rows(a, g, x.r0, x.r1);
+  x.chunks = (min(x.r1 - x.r0, a.max_rows) * a.G + (1 << a.rows_shift) - 1) >> a.rows_shift;
+  x.pages = x.chunks > 0 ? min(max(n, 0), a.max_blocks) : 0;
+  return x;
 }
 
-// Sets lo: the first shared page inside every row's window (uniform over the wave).
-__device__ inline void window_start(const RowArgs& a, SharedPages& s, int r0, int r1, int lane) {
-  if (a.window <= 0) return;
-  int longest = 0;
-  for (int r = r0 + lane; r < r1; r += 64) longest = max(longest, a.ctx[r]);
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) longest = max(longest, __shfl_xor(longest, o));
-  s.lo = min(s.blocks, max(s.base, cdiv(max(uni(longest) - a.window, 0), kBS)));
+// Whether a sequence of length len takes part in its group's shared walk of `blocks` pages: it has
+// the whole prefix and its window cuts nothing off.  (Any other row walks all of its visible pages
+// itself, so the shared walk needs no mask of its own.)
+__device__ inline bool takes_part(const RowArgs& a, int len, int blocks) {
+  return len >= blocks * kBS && (a.window <= 0 || len <= a.window);
 }
 
-// The first row of [r0, r1) that has the whole prefix, whose table the shared walk reads (-1: none, and
-// then no row asks for the walk's partials).
-__device__ inline int prefix_row(const RowArgs& a, const SharedPages& s, int r0, int r1, int lane) {
+// The first row of [r0, r1) that takes part, whose table the shared walk reads (-1: none, and then no
+// row asks for the walk's partials).
+__device__ inline int prefix_row(const RowArgs& a, int blocks, int r0, int r1, int lane) {
   for (int r = r0; r < r1; r += 64) {
-    const uint64_t has = __builtin_amdgcn_ballot_w64(r + lane < r1 && a.ctx[min(r + lane, r1 - 1)] >= s.blocks * kBS);
+    const uint64_t has =
+        __builtin_amdgcn_ballot_w64(r + lane < r1 && takes_part(a, a.ctx[min(r + lane, r1 - 1)], blocks));
     if (has != 0) return r + __builtin_ctzll(has);
   }
   return -1;
 }
 
-// List entries (pages) of group g, -1 for a group without rows.
-__device__ inline int group_pages(const RowArgs& a, int g) {
-  int r0, r1;
-  group_rows(a, g, r0, r1);
-  if (r1 <= r0) return -1;
-  if (a.prefix) return shared_pages(a, g).listed();
-  const int n = a.ctx[g];
-  return min(cdiv(n < 0 ? 0 : n, kBS), a.max_blocks);
+// Inclusive scan over the wave's lanes (row shifts, then the rows' last lanes broadcast).
+__device__ inline int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);
+  return x;
 }
+__device__ inline int wave_sum(int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
 
-// Segments: every group's list is cut into pieces of `len` pages, a multiple of the eight pages that
-// a workgroup's waves take at once, sized so that all groups' pieces number at most `segments`:
-// whole pieces are at most segments - n_groups, and a group has at most one that is not whole.
-// A cross group without keys has one empty piece, which writes its rows' zeros.
-struct Segments {
-  int len, least;
-  __device__ inline int of(int pages) const { return pages < 0 ? 0 : max((pages + len - 1) / len, least); }
+// How the groups' pages are cut: every list into pieces of `len` pages (a multiple of the pages that a
+// workgroup's waves take at once), the shortest of four lengths with which all groups' items, pieces
+// times row chunks, number at most a.items.  The last of the four, sum (pages x chunks) / (items -
+// sum chunks), always does: a group has at most one piece that is not whole.  Without a.split
+// every group is one piece.  Partials, and the shared workgroups, are numbered group by group, in it
+// piece by piece, kv head by kv head, chunk by chunk.  A cross group without keys has one empty
+// piece, which writes its rows' zeros.  Each wave works this out for itself, 64 groups at a time,
+// the first 64 (`own`, group `lane`) from registers.
+struct Pieces {
+  int len, least, items;  // items: of all groups
+  __device__ inline int of(const Group& x) const {
+    return x.chunks == 0 ? 0 : max((int)(((uint32_t)x.pages + (uint32_t)len - 1) / (uint32_t)len), least);
+  }
+
+  __device__ inline Pieces(const RowArgs& a, const Group& own, int lane) {
+    least = a.prefix ? 0 : 1;
+    len = 1 << 30;
+    int work = 0, chunks = 0;
+    if (a.split) {  // (then items x max_blocks, and so the work, is below 2^31)
+      work = wave_sum(own.pages * own.chunks);
+      chunks = wave_sum(own.chunks);
+      for (int g0 = 64; g0 < a.n_groups; g0 += 64) {
+        const Group x = load_group(a, g0 + lane);
+        work += wave_sum(x.pages * x.chunks);
+        chunks += wave_sum(x.chunks);
+      }
+    }
+#pragma unroll 1
+    for (int k = a.split ? 0 : 3; k < 4; ++k) {
+      if (a.split) {
+        const uint32_t parts = (uint32_t)max(a.items - k * chunks / 3, 1), unit = (uint32_t)a.unit;
+        len = (int)max(((uint32_t)work + parts * unit - 1) / (parts * unit) * unit, unit);
+      }
+      items = wave_sum(of(own) * own.chunks);
+      for (int g0 = 64; g0 < a.n_groups; g0 += 64) {
+        const Group x = load_group(a, g0 + lane);
+        items += wave_sum(of(x) * x.chunks);
+      }
+      if (items <= a.items) return;
+    }
+  }
+
+  // What shared workgroup `wg` does: the group, which of its pieces, kv head and chunk; false when
+  // there is nothing for it.
+  __device__ inline bool find(const RowArgs& a, const Group& own, int wg, int lane, Group& group, int& g, int& piece,
+                              int& h, int& chunk) const {
+    int before = 0;
+    for (int g0 = 0; g0 < a.n_groups; g0 += 64) {
+      const Group x = g0 == 0 ? own : load_group(a, g0 + lane);
+      const int n = of(x) * x.chunks * a.Hkv, incl = wave_scan(n);
+      const uint64_t has = __builtin_amdgcn_ballot_w64(wg < before + incl);
+      if (has != 0) {
+        const int w = __builtin_ctzll(has);
+        g = g0 + w;
+        group = Group{__builtin_amdgcn_readlane(x.r0, w), __builtin_amdgcn_readlane(x.r1, w),
+                      __builtin_amdgcn_readlane(x.chunks, w), __builtin_amdgcn_readlane(x.pages, w)};
+        const uint32_t at = (uint32_t)(wg - before - (__builtin_amdgcn_readlane(incl, w) - __builtin_amdgcn_readlane(n, w)));
+        chunk = (int)(at % (uint32_t)group.chunks);
+        const uint32_t ph = at / (uint32_t)group.chunks;
+        h = (int)(ph % (uint32_t)a.Hkv);
+        piece = (int)(ph / (uint32_t)a.Hkv);
+        return true;
+      }
+      before += __builtin_amdgcn_readlane(incl, 63);
+    }
+    return false;
+  }
+
+  // First partial of group g, and its pieces.
+  __device__ inline void of_group(const RowArgs& a, const Group& own, int g, int lane, int64_t& first,
+                                  int& pieces) const {
+    int before = 0, n = 0, mine = 0;
+    for (int g0 = 0; g0 <= g; g0 += 64) {
+      const Group x = g0 == 0 ? own : load_group(a, g0 + lane);
+      mine = of(x);
+      n = g0 + lane <= g ? mine * x.chunks : 0;
+      before += wave_sum(n);
+    }
+    pieces = __builtin_amdgcn_readlane(mine, g & 63);
+    first = (int64_t)(before - __builtin_amdgcn_readlane(n, g & 63)) * a.Hkv;
+  }
 };
 
-// The segment length: each wave sums the groups' pages, 64 at a time.
-__device__ inline Segments segment_len(const RowArgs& a, int lane) {
-  int64_t total = 0;
-  for (int g0 = 0; g0 < a.n_groups; g0 += 64) {
-    int n = g0 + lane < a.n_groups ? max(group_pages(a, g0 + lane), 0) : 0;
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) n += __shfl_xor(n, o);
-    total += uni(n);
-  }
-  const int parts = max(a.segments - a.n_groups, 1);
-  const int64_t len = (total + parts - 1) / parts;
-  Segments s;
-  s.len = (int)min<int64_t>(max<int64_t>((len + 7) & ~7ll, 8), 1 << 28);
-  s.least = a.prefix ? 0 : 1;
-  return s;
-}
+// Workgroups of the walks: four waves of 256 registers, two workgroups per CU (a shared one and one
+// of the own walk, say); rows of 512 bytes need 512 registers.
+template <int DT, int D, bool kFp8, int NR>
+struct Shape {
+  static constexpr int kRow = D * (DT == IVAKV_F32 ? 4 : 2);  // bytes of a query row
+  static constexpr bool kWide = kRow >= 512;
+  static constexpr int W = 4;
+  static constexpr int kRegs = kWide ? 512 : 256;
+  using WalkT = Walk<DT, D, kFp8, NR, kRegs>;
+  static constexpr int kLds = (int)(join_floats<D, NR, W>() * sizeof(float)) + WalkT::kQBytes;
+};
 
-// The group of segment `seg` and which piece of the group it is (group -1: no such segment).
-__device__ inline void find_segment(const RowArgs& a, const Segments& sg, int seg, int lane, int& group,
-                                    int& piece) {
-  int before = 0;
-  group = -1;
-  piece = 0;
-  for (int g0 = 0; g0 < a.n_groups; g0 += 64) {
-    const int n = g0 + lane < a.n_groups ? sg.of(group_pages(a, g0 + lane)) : 0;
-    int incl = n;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int u = __shfl_up(incl, o);
-      if (lane >= o) incl += u;
-    }
-    const uint64_t has = __builtin_amdgcn_ballot_w64(seg < before + incl);
-    if (has != 0) {
-      const int w = __builtin_ctzll(has);
-      group = g0 + w;
-      piece = seg - before - (__shfl(incl, w) - __shfl(n, w));
-      return;
-    }
-    before += __shfl(incl, 63);
-  }
-}
-
-// First segment of group g, and how many it has.
-__device__ inline void group_segments(const RowArgs& a, const Segments& sg, int group, int lane, int& first,
-                                      int& count) {
-  int before = 0;
-  count = 0;
-  for (int g0 = 0; g0 <= group; g0 += 64) {
-    const int n = g0 + lane <= group ? sg.of(group_pages(a, g0 + lane)) : 0;
-    int sum = n;
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
-    before += sum;
-    if (group < g0 + 64) count = __shfl(n, group - g0);
-  }
-  first = uni(before - count);
-  count = uni(count);
-}
-
-// Slot of a partial: segment, kv head, row chunk.
-__device__ inline int64_t slot_of(const RowArgs& a, int seg, int h, int chunk) {
-  return ((int64_t)seg * a.Hkv + h) * a.chunks + chunk;
-}
-
-// Shared walk.  Grid: (segment, kv head) x row chunk, a pair's chunks on one XCD (ids equal mod 8)
-// one after the other, so that chunks past the first find the pages in its L2.
+// One segment of one group for a chunk of rows.
 template <int DT, int D, bool kFp8, int NR, bool NT>
-__global__ __launch_bounds__(kThreads) void rows_walk_kernel(RowArgs a, const int32_t* __restrict__ bt) {
-  using WalkT = Walk<DT, D, kFp8, NR>;
+__device__ inline void shared_walk(const RowArgs& a, const int32_t* __restrict__ bt, int wg, float* smem,
+                                   float* s_fin) {
+  using S = Shape<DT, D, kFp8, NR>;
+  using WalkT = typename S::WalkT;
   using E = typename WalkT::E;
-  constexpr int R = 16 * NR;
-  extern __shared__ float smem[];
-  __shared__ float s_fin[2 * R];
-  const int xcd = blockIdx.x & 7, at = blockIdx.x >> 3;
-  const int chunk = at % a.chunks, sh = (at / a.chunks) * 8 + xcd;
-  if (sh >= a.segments * a.Hkv) return;
-  const int seg = sh / a.Hkv, h = sh % a.Hkv;
+  constexpr int R = 16 * NR, W = S::W;
   const int lane = threadIdx.x & 63, ln = lane & 15, lq = lane >> 4;
   const int wave = uni(threadIdx.x >> 6);
-  const Segments sg = segment_len(a, lane);
-  int g, piece;
-  find_segment(a, sg, seg, lane, g, piece);
-  g = uni(g);
-  piece = uni(piece);
-  if (g < 0) return;
-  int r0, r1;
-  group_rows(a, g, r0, r1);
-  const int rows = (r1 - r0) * a.G;  // (at most 2^31 / Hkv: the entry checks n_rows * Hq)
-  if (chunk * R >= rows) return;
+  const Group own = load_group(a, lane);
+  const Pieces pc(a, own, lane);
+  // Each XCD takes a contiguous run of the workgroups, so that a piece's chunks are on one XCD, one
+  // after the other: chunks past the first find the pages in its L2.
+  const int n_wg = pc.items * a.Hkv;
+  if (wg >= n_wg) return;
+  wg = (int)xcd_contiguous_block(wg, n_wg);
+  Group group;
+  int g, piece, h, chunk;
+  if (!pc.find(a, own, wg, lane, group, g, piece, h, chunk)) return;
+  const int rows = min(group.r1 - group.r0, a.max_rows) * a.G;  // (at most n_rows * Hq, which the entry checks)
   KeyList kl;
   kl.num_pages = a.num_pages;
-  kl.win_start = kl.n_sink = kl.a0 = kl.na = kl.b0 = kl.nb = 0;
-  int n;
-  if (a.prefix) {
-    SharedPages s = shared_pages(a, g);
-    window_start(a, s, r0, r1, lane);
-    const int row = prefix_row(a, s, r0, r1, lane);
-    if (row < 0) return;
-    n = s.listed();
-    kl.row = bt + (int64_t)row * a.max_blocks;
-    kl.na = s.sinks;
-    kl.c0 = s.base;
-    kl.len = s.blocks * kBS;
-    // pages [base, lo) of the list are left to the rows' own walks
-    kl.win_start = s.lo * kBS;
-    kl.n_sink = s.sinks * kBS;
-  } else {
-    n = group_pages(a, g);
-    kl.row = bt + (int64_t)g * a.max_blocks;
-    kl.c0 = 0;
-    kl.len = a.ctx[g];
-  }
-  const int v0 = piece * sg.len, v1 = min(v0 + sg.len, n);
+  kl.win_start = kl.n_sink = kl.na = kl.c0 = 0;
+  int table = g;
+  kl.len = group.pages * kBS;
+  if (a.prefix) table = prefix_row(a, group.pages, group.r0, group.r1, lane);
+  else kl.len = a.ctx[g];
+  if (table < 0) return;
+  kl.row = bt + (int64_t)table * a.max_blocks;
+  const int v0 = piece * pc.len, v1 = min(v0 + pc.len, group.pages);
   WalkT wk;
-  wk.init(a, r0, rows, h, chunk * R, ln, lq);
-  wk.template run<NT, kWaves>(a, kl, h, v0, v1, wave, ln, lq);
-  join_waves<WalkT, D, NR, kWaves>(wk, smem, wave, ln, lq, s_fin);
-  const float* s_acc = smem + 2 * kWaves * R;
-  const bool whole = !a.prefix && sg.of(n) == 1;
-  const int64_t slot = slot_of(a, seg, h, chunk);
+  wk.template init<W>(a, group.r0, rows, h, chunk * R, wave, ln, lq,
+                      reinterpret_cast<Chunk16*>(smem + join_floats<D, NR, W>()));
+  wk.template run<NT, W>(a, kl, h, v0, v1, wave, ln, lq);
+  join_waves<WalkT, D, NR, W>(wk, smem, wave, ln, lq, s_fin);
+  const float* s_acc = smem + 2 * W * R;
+  const bool whole = !a.prefix && pc.of(group) == 1;
+  const int64_t slot = wg;
   const int Hq = a.Hkv * a.G;
-  for (int e = threadIdx.x; e < R * (D / 4); e += kThreads) {
+  for (int e = threadIdx.x; e < R * (D / 4); e += 64 * W) {
     const int row = e / (D / 4), d = 4 * (e % (D / 4)), r = chunk * R + row;
     if (r >= rows) break;
     f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int u = 0; u < kWaves; ++u) o += *reinterpret_cast<const f32x4*>(s_acc + (u * R + row) * (D + 4) + d);
+    for (int u = 0; u < W; ++u) o += *reinterpret_cast<const f32x4*>(s_acc + (u * R + row) * (D + 4) + d);
     if (whole) {
       const float L = s_fin[2 * row + 1], inv = L > 0.f ? 1.f / L : 0.f;
-      E* dst = static_cast<E*>(a.out) + ((int64_t)(r0 + r / a.G) * Hq + h * a.G + r % a.G) * D + d;
+      E* dst = static_cast<E*>(a.out) + ((int64_t)(group.r0 + r / a.G) * Hq + h * a.G + r % a.G) * D + d;
 #pragma unroll
       for (int i = 0; i < 4; ++i) dst[i] = WalkT::Tr::from_float(o[i] * inv);
     } else {
@@ -743,36 +760,190 @@ __global__ __launch_bounds__(kThreads) void rows_walk_kernel(RowArgs a, const in
   }
 }
 
-// Log-sum-exp fold of the partials of segments [first, first + count) of row r (kv head h) at
-// elements d .. d + 3 into (M, L, O), U at a time.
-template <int D>
-__device__ inline void fold_segments(const RowArgs& a, int first, int count, int h, int r, int d, float& M,
+// The group that query row `row` (of this thread) belongs to: its pages (0: none) and first row.
+__device__ inline int row_pages(const RowArgs& a, int row, int& r0) {
+  int lo = 0, hi = a.n_groups;  // the last group that starts at or before the row
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (a.start[mid] <= row) lo = mid + 1;
+    else hi = mid;
+  }
+  r0 = 0;
+  if (lo == 0) return 0;
+  const Group x = load_group(a, lo - 1);
+  if (row < x.r0 || row >= x.r1 || row - x.r0 >= a.max_rows) return 0;
+  r0 = x.r0;
+  return x.pages;
+}
+
+// A sequence's own pages: of one that takes part in a shared walk those after the prefix, else all that
+// its window and sinks leave.  `blocks`: shared pages of its group, 0 when it has none.
+struct OwnPages {
+  KeyList kl;
+  int n;
+  bool part;
+  __device__ inline OwnPages(const RowArgs& a, int len, int blocks) {
+    const PageWalk w = make_walk(len, a.window, a.n_sink, kBS);
+    part = blocks > 0 && takes_part(a, len, blocks);
+    kl.len = w.L;
+    kl.num_pages = a.num_pages;
+    if (part) {
+      kl.win_start = kl.n_sink = kl.na = 0;
+      kl.c0 = blocks;
+      n = max(min(cdiv(w.L, kBS), a.max_blocks) - blocks, 0);
+    } else {
+      kl.win_start = w.win_start;
+      kl.n_sink = a.n_sink;
+      kl.na = w.sink_pages;
+      kl.c0 = w.win_first;
+      n = table_pages(w, a.max_blocks, kBS);
+    }
+  }
+};
+
+// Own walk: tile t of T is a set of PG own pages, in the order (sequence, kv head, set); wave k of W
+// owns tiles [k T / W, (k + 1) T / W).  What it leaves of unit u (sequence * Hkv + kv head) goes to
+// own slot k + u, which rises along the tiles.
+struct OwnSplit {
+  uint32_t T, W;
+  __device__ inline OwnSplit(uint32_t tiles, const RowArgs& a) : T(tiles) {
+    // two tiles a wave at least: a walk of one has nothing in flight beside it
+    W = min(max((T + 1) / 2, 1u), (uint32_t)a.own_waves);
+  }
+  __device__ inline uint32_t start(uint32_t k) const { return div((uint64_t)k * T, W); }
+  // The wave k with start(k) <= t < start(k + 1).
+  __device__ inline uint32_t owner(uint32_t t) const { return div((uint64_t)(t + 1) * W - 1, T); }
+  // (a 64-bit division takes long on the walk's way to its first load)
+  static __device__ inline uint32_t div(uint64_t x, uint32_t y) {
+    return x >> 32 == 0 ? (uint32_t)x / y : (uint32_t)(x / y);
+  }
+};
+
+template <int DT, int D, bool kFp8, int kRegs>
+__device__ inline void own_walk(const RowArgs& a, const int32_t* __restrict__ bt, int wg, int32_t* s_pref) {
+  using WalkT = Walk<DT, D, kFp8, 1, kRegs>;
+  constexpr int PG = WalkT::PG, W = 4;
+  const int lane = threadIdx.x & 63, ln = lane & 15, lq = lane >> 4;
+  const int wave = uni(threadIdx.x >> 6);
+  __shared__ int s_wave[W];
+  // Prefix of the sequences' sets (a contiguous run per thread, a scan per wave, the waves' totals), with
+  // their shared pages packed beside: s_pref[b] sets before b, s_pref[n + 1 + b] pages it shares.
+  const int n = a.n_rows, each = (n + 64 * W - 1) / (64 * W);
+  const int b0 = min((int)threadIdx.x * each, n), b1 = min(b0 + each, n);
+  int mine = 0;
+  for (int b = b0; b < b1; ++b) {
+    int r0;
+    const int blocks = row_pages(a, b, r0);
+    const OwnPages own(a, a.ctx[b], blocks);
+    const int sets = (own.n + PG - 1) / PG;
+    s_pref[b + 1] = sets;
+    s_pref[n + 1 + b] = own.part ? blocks : 0;
+    mine += sets;
+  }
+  const int incl = wave_scan(mine);
+  if (lane == 63) s_wave[wave] = incl;
+  __syncthreads();
+  int run = incl - mine;
+  for (int w = 0; w < wave; ++w) run += s_wave[w];
+  if (threadIdx.x == 0) s_pref[0] = 0;
+  for (int b = b0; b < b1; ++b) {
+    run += s_pref[b + 1];
+    s_pref[b + 1] = run;
+  }
+  __syncthreads();
+  if (wg == 0)
+    for (int b = threadIdx.x; b <= n; b += 64 * W) a.own_pref[b] = s_pref[b];
+  const uint32_t T = (uint32_t)uni(s_pref[n]) * (uint32_t)a.Hkv;
+  if (T == 0) return;
+  const OwnSplit split(T, a);
+  const uint32_t k = (uint32_t)(wg * W + wave);
+  if (k >= split.W) return;
+  uint32_t t = split.start(k);
+  const uint32_t end = split.start(k + 1);
+  const int Hq = a.Hkv * a.G;
+  // the last sequence with s_pref <= t / Hkv (it has sets)
+  int b = 0, hi = n;
+  const int key = (int)(t / (uint32_t)a.Hkv);
+  while (hi - b > 1) {
+    const int mid = (b + hi) >> 1;
+    if (s_pref[mid] <= key) b = mid;
+    else hi = mid;
+  }
+  b = uni(b);
+  while (t < end) {
+    while (s_pref[b + 1] == s_pref[b]) ++b;  // (a sequence without sets: some later one has, as t < T)
+    b = uni(b);
+    const uint32_t sets = (uint32_t)uni(s_pref[b + 1] - s_pref[b]), base = (uint32_t)uni(s_pref[b]) * (uint32_t)a.Hkv;
+    const int h = (int)((t - base) / sets);
+    const uint32_t first = base + (uint32_t)h * sets, stop = min(end, first + sets);
+    OwnPages own(a, a.ctx[b], uni(s_pref[n + 1 + b]));
+    own.kl.row = bt + (int64_t)b * a.max_blocks;
+    const int v0 = (int)(t - first) * PG, v1 = min((int)(stop - first) * PG, own.n);
+    const int64_t slot = (int64_t)k + (int64_t)b * a.Hkv + h;
+    for (int g0 = 0; g0 < a.G; g0 += 16) {
+      WalkT wk;
+      wk.template init<1>(a, b, a.G, h, g0, 0, ln, lq, nullptr);
+      wk.template run<true, 1>(a, own.kl, h, v0, v1, 0, ln, lq);
+      const float l = wk.total(0);
+      if (g0 + ln < a.G) {
+        float* dst = a.own_acc + (slot * a.G + g0 + ln) * D + 4 * lq;
+#pragma unroll
+        for (int m = 0; m < D / 16; ++m) *reinterpret_cast<f32x4*>(dst + 16 * m) = wk.acc[0][m];
+        if (lq == 0) *reinterpret_cast<f32x2*>(a.own_ml + (slot * a.G + g0 + ln) * 2) = f32x2{wk.m[0], l};
+      }
+    }
+    t = stop;
+    if (h == a.Hkv - 1 && stop == first + sets) ++b;
+  }
+}
+
+// The walks: workgroups [0, shared_wgs) the shared segments, the others the own pages.
+template <int DT, int D, bool kFp8, int NR, bool NT>
+__global__ __launch_bounds__(256, (512 / Shape<DT, D, kFp8, NR>::kRegs)) void rows_walk_kernel(
+    RowArgs a, const int32_t* __restrict__ bt) {
+  extern __shared__ __align__(16) float smem[];
+  __shared__ float s_fin[32 * NR];
+  if ((int)blockIdx.x < a.shared_wgs) shared_walk<DT, D, kFp8, NR, NT>(a, bt, blockIdx.x, smem, s_fin);
+  else own_walk<DT, D, kFp8, Shape<DT, D, kFp8, NR>::kRegs>(a, bt, blockIdx.x - a.shared_wgs,
+                                                              reinterpret_cast<int32_t*>(smem));
+}
+
+// Log-sum-exp fold of one more state into (M, L, O).
+__device__ inline void fold_state(float& M, float& L, f32x4& O, float m, float l, const f32x4& o) {
+  const float mc = fmaxf(M, m), m_use = mc == kNegInf ? 0.f : mc;
+  const float fa = exp2_fast(M - m_use), fb = exp2_fast(m - m_use);
+  L = L * fa + l * fb;
+  O = O * fa + o * fb;
+  M = mc;
+}
+
+// Log-sum-exp fold of `count` partials at(i) (state index of a row) at elements d .. d + 3 into
+// (M, L, O), U at a time.
+template <int D, class At>
+__device__ inline void fold_partials(const float* acc, const float* mls, int count, int d, At at, float& M,
                                      float& L, f32x4& O) {
-  constexpr int U = 4;
-  const int chunk = r / a.rows_chunk, row = r % a.rows_chunk;
+  constexpr int U = 8;
   for (int s0 = 0; s0 < count; s0 += U) {
-    float mv[U], lv[U];
+    f32x2 ml[U];
     f32x4 av[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int64_t at = slot_of(a, first + min(s0 + u, count - 1), h, chunk) * a.rows_chunk + row;
-      const f32x2 ml = *reinterpret_cast<const f32x2*>(a.part_ml + at * 2);
-      mv[u] = s0 + u < count ? ml[0] : kNegInf;
-      lv[u] = ml[1];
-      av[u] = *reinterpret_cast<const f32x4*>(a.part_acc + at * D + d);
+      const int64_t i = at(min(s0 + u, count - 1));
+      ml[u] = *reinterpret_cast<const f32x2*>(mls + i * 2);
+      av[u] = *reinterpret_cast<const f32x4*>(acc + i * D + d);
     }
     float mc = M;
 #pragma unroll
-    for (int u = 0; u < U; ++u) mc = fmaxf(mc, mv[u]);
+    for (int u = 0; u < U; ++u) mc = fmaxf(mc, ml[u][0]);  // (a repeated one changes no max)
     const float m_use = mc == kNegInf ? 0.f : mc;
     const float f = exp2_fast(M - m_use);
     L *= f;
     O *= f;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const float w = exp2_fast(mv[u] - m_use);
+      const float w = exp2_fast(ml[u][0] - m_use);
       if (s0 + u < count) {
-        L += lv[u] * w;
+        L += ml[u][1] * w;
         O += av[u] * w;
       }
     }
@@ -780,209 +951,209 @@ __device__ inline void fold_segments(const RowArgs& a, int first, int count, int
   }
 }
 
-// The group that query row `row` belongs to and the group's rows; false when there is none, or the
-// row lies past the largest group the launch was sized for (uniform over the wave).
-__device__ inline bool row_group(const RowArgs& a, int row, int lane, int& g, int& r0, int& r1) {
-  g = -1;
-  for (int g0 = 0; g0 < a.n_groups; g0 += 64) {  // the last group that starts at or before it
-    const uint64_t le = __builtin_amdgcn_ballot_w64(g0 + lane < a.n_groups && a.start[min(g0 + lane, a.n_groups)] <= row);
-    if (le == 0) break;
-    g = g0 + 63 - __builtin_clzll(le);
-  }
-  r0 = r1 = 0;
-  if (g < 0) return false;
-  group_rows(a, g, r0, r1);
-  return row >= r0 && row < r1 && row - r0 < a.max_rows;
-}
-
-// Cross attention's second launch: rows of groups cut into more than one segment.  Grid (kv head,
-// query row).
+// The join: a workgroup per (query row, kv head).  Its elements (four dims of a head) are dealt to
+// as many threads each as there are, every one folding a run of the row's partials.
 template <int DT, int D>
-__global__ __launch_bounds__(kThreads) void rows_merge_kernel(RowArgs a) {
+__global__ __launch_bounds__(256) void rows_join_kernel(RowArgs a) {
   using E = typename Traits<DT>::E;
-  const int h = blockIdx.x % a.Hkv, row = blockIdx.x / a.Hkv, lane = threadIdx.x & 63;
-  int g, r0, r1;
-  if (!row_group(a, row, lane, g, r0, r1)) return;
-  const Segments sg = segment_len(a, lane);
-  int first, count;
-  group_segments(a, sg, g, lane, first, count);
-  if (count == 1) return;  // written by the walk
-  const int Hq = a.Hkv * a.G;
-  for (int e = threadIdx.x; e < a.G * (D / 4); e += kThreads) {
-    const int head = e / (D / 4), d = 4 * (e % (D / 4));
-    float M = kNegInf, L = 0.f;
-    f32x4 O = f32x4{0.f, 0.f, 0.f, 0.f};
-    fold_segments<D>(a, first, count, h, (row - r0) * a.G + head, d, M, L, O);
-    const float inv = L > 0.f ? 1.f / L : 0.f;
-    E* dst = static_cast<E*>(a.out) + ((int64_t)row * Hq + h * a.G + head) * D + d;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) dst[i] = Traits<DT>::from_float(O[i] * inv);
-  }
-}
-
-// The prefix op's second launch: a workgroup walks one sequence's own pages for up to 16 heads of
-// a kv head and joins the shared segments' partials.  Grid (kv head x block of 16 heads, sequence).
-template <int DT, int D, bool kFp8, int W>
-__global__ __launch_bounds__(64 * W) void prefix_own_kernel(RowArgs a, const int32_t* __restrict__ bt) {
-  using WalkT = Walk<DT, D, kFp8, 1>;
-  using E = typename WalkT::E;
-  extern __shared__ float smem[];
-  __shared__ float s_fin[32];
-  const int head_blocks = (a.G + 15) / 16, per_row = a.Hkv * head_blocks;
-  const int b = blockIdx.x / per_row, h = blockIdx.x % per_row / head_blocks, g0 = 16 * (blockIdx.x % head_blocks);
-  const int lane = threadIdx.x & 63, ln = lane & 15, lq = lane >> 4;
-  const int wave = uni(threadIdx.x >> 6);
-  const int L = max(a.ctx[b], 0);
-  int g, r0, r1, first = 0, count = 0;
-  SharedPages s{0, 0, 0, 0};
-  if (row_group(a, b, lane, g, r0, r1)) {
-    s = shared_pages(a, g);
-    if (L >= s.blocks * kBS) {
-      window_start(a, s, r0, r1, lane);
-      group_segments(a, segment_len(a, lane), g, lane, first, count);
-    } else {
-      s = SharedPages{0, 0, 0, 0};  // shorter than the prefix: its own walk takes everything
+  __shared__ float smem[6 * 256];
+  const int h = blockIdx.x % a.Hkv, row = blockIdx.x / a.Hkv, lane = threadIdx.x & 63, tid = threadIdx.x;
+  const Group mine = load_group(a, lane);
+  // the group of the row (uniform)
+  int g = -1, r0 = 0, pages = 0, chunks = 0;
+  for (int g0 = 0; g0 < a.n_groups && g < 0; g0 += 64) {
+    const Group x = g0 == 0 ? mine : load_group(a, g0 + lane);
+    const uint64_t in = __builtin_amdgcn_ballot_w64(x.r0 <= row && row < x.r1);
+    if (in != 0) {
+      const int w = __builtin_ctzll(in);
+      g = g0 + w;
+      r0 = __builtin_amdgcn_readlane(x.r0, w);
+      pages = __builtin_amdgcn_readlane(x.pages, w);
+      chunks = __builtin_amdgcn_readlane(x.chunks, w);
     }
   }
-  // Own pages: the sink pages before the window, then the window's, without those of the shared
-  // walk, [0, sinks) and [lo, blocks).
-  const PageWalk w = make_walk(L, a.window, a.n_sink, kBS);
-  const int n_log = min(cdiv(L, kBS), a.max_blocks);
-  KeyList kl;
-  kl.row = bt + (int64_t)b * a.max_blocks;
-  kl.num_pages = a.num_pages;
-  kl.len = L;
-  kl.win_start = w.win_start;
-  kl.n_sink = a.n_sink;
-  kl.a0 = s.sinks;
-  kl.na = max(min(w.sink_pages, n_log) - s.sinks, 0);
-  kl.b0 = w.win_first;
-  kl.nb = max(min(s.lo, n_log) - w.win_first, 0);
-  kl.c0 = max(w.win_first, s.blocks);
-  const int n = kl.na + kl.nb + max(n_log - kl.c0, 0);
-  WalkT wk;
-  wk.init(a, b, a.G, h, g0, ln, lq);
-  wk.template run<true, W>(a, kl, h, 0, n, wave, ln, lq);
-  join_waves<WalkT, D, 1, W>(wk, smem, wave, ln, lq, s_fin);
-  const float* s_acc = smem + 2 * W * 16;
-  const int heads = min(a.G - g0, 16), Hq = a.Hkv * a.G;
-  for (int e = threadIdx.x; e < heads * (D / 4); e += 64 * W) {
-    const int head = e / (D / 4), d = 4 * (e % (D / 4));
-    f32x4 O = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int u = 0; u < W; ++u) O += *reinterpret_cast<const f32x4*>(s_acc + (u * 16 + head) * (D + 4) + d);
-    float M = s_fin[2 * head], Ls = s_fin[2 * head + 1];
-    fold_segments<D>(a, first, count, h, (b - r0) * a.G + g0 + head, d, M, Ls, O);
-    const float inv = Ls > 0.f ? 1.f / Ls : 0.f;
-    E* dst = static_cast<E*>(a.out) + ((int64_t)b * Hq + h * a.G + g0 + head) * D + d;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) dst[i] = WalkT::Tr::from_float(O[i] * inv);
+  if (g >= 0 && row - r0 >= a.max_rows) g = -1;
+  int64_t first = 0;
+  int count = 0;
+  if (!a.prefix) {
+    if (g < 0) return;  // no sequence's row, or one the launch was not sized for: left as it is
+    Pieces(a, mine, lane).of_group(a, mine, g, lane, first, count);
+    if (count == 1) return;  // written by the walk
+  } else if (g >= 0 && pages > 0 && takes_part(a, a.ctx[row], pages)) {
+    Pieces(a, mine, lane).of_group(a, mine, g, lane, first, count);
   }
+  // the own walk's partials: slots k + u of the waves that had tiles of this unit
+  int64_t own_first = 0;
+  int own_count = 0;
+  if (a.own_waves > 0) {
+    const uint32_t p0 = (uint32_t)a.own_pref[row], p1 = (uint32_t)a.own_pref[row + 1];
+    const uint32_t T = (uint32_t)a.own_pref[a.n_rows] * (uint32_t)a.Hkv, sets = p1 - p0;
+    if (sets > 0) {
+      const OwnSplit split(T, a);
+      const uint32_t t0 = p0 * (uint32_t)a.Hkv + (uint32_t)h * sets;
+      const uint32_t k0 = split.owner(t0), k1 = split.owner(t0 + sets - 1);
+      own_first = (int64_t)k0 + (int64_t)row * a.Hkv + h;
+      own_count = (int)(k1 - k0) + 1;
+    }
+  }
+  const int n_el = a.G * (D / 4), total = count + own_count;
+  E* out = static_cast<E*>(a.out) + ((int64_t)row * a.Hkv + h) * a.G * D;
+  int split = 1;
+  while (split < 16 && 2 * split * n_el <= 256 && split < total) split *= 2;
+  // partials [i0, i1) of one element: the shared ones, then the own
+  auto fold = [&](int e, int i0, int i1, float& M, float& L, f32x4& O) IVAKV_INLINE {
+    const int head = e / (D / 4), d = 4 * (e % (D / 4)), r = (row - r0) * a.G + head;
+    const int at = r & ((1 << a.rows_shift) - 1);
+    const int64_t slot = first + (int64_t)h * chunks + (r >> a.rows_shift), step = (int64_t)a.Hkv * chunks;
+    const int s1 = min(i1, count), o0 = max(i0 - count, 0);
+    fold_partials<D>(a.part_acc, a.part_ml, s1 - i0, d,
+                     [&](int i) { return ((slot + (i0 + i) * step) << a.rows_shift) + at; }, M, L, O);
+    fold_partials<D>(a.own_acc, a.own_ml, i1 - count - o0, d,
+                     [&](int i) { return (own_first + o0 + i) * a.G + head; }, M, L, O);
+  };
+  auto emit = [&](int e, float L, const f32x4& O) IVAKV_INLINE {
+    const float inv = L > 0.f ? 1.f / L : 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[4 * e + i] = Traits<DT>::from_float(O[i] * inv);
+  };
+  if (split == 1) {
+    for (int e = tid; e < n_el; e += 256) {
+      float M = kNegInf, L = 0.f;
+      f32x4 O = f32x4{0.f, 0.f, 0.f, 0.f};
+      fold(e, 0, total, M, L, O);
+      emit(e, L, O);
+    }
+    return;
+  }
+  const int e = tid % n_el, part = tid / n_el, each = (total + split - 1) / split;
+  float M = kNegInf, L = 0.f;
+  f32x4 O = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (part < split) fold(e, min(part * each, total), min((part + 1) * each, total), M, L, O);
+  if (part > 0 && part < split) {
+    smem[6 * tid] = M;
+    smem[6 * tid + 1] = L;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) smem[6 * tid + 2 + i] = O[i];
+  }
+  __syncthreads();
+  if (part > 0) return;
+  for (int p = 1; p < split; ++p) {
+    const float* x = smem + 6 * (tid + p * n_el);
+    fold_state(M, L, O, x[0], x[1], f32x4{x[2], x[3], x[4], x[5]});
+  }
+  emit(e, L, O);
 }
 
-// Row blocks of a wave: as many as the rows need, up to what the registers hold beside two sets
-// of pages in flight.
-constexpr int max_row_blocks(bool fp8, int d) {
-  return fp8 ? (d == 256 ? 2 : 4) : d == 64 ? 4 : d == 128 ? 2 : 1;
-}
-int row_blocks(bool fp8, int d, int64_t rows) {
-  const int most = max_row_blocks(fp8, d);
-  const int want = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+// Row blocks of a wave: as many as the rows need, up to what the registers hold beside the pages in
+// flight.
+constexpr int max_row_blocks(int row_bytes) { return row_bytes >= 1024 ? 1 : row_bytes >= 256 ? 2 : 4; }
+int row_blocks(int row_bytes, int64_t rows) {
+  const int most = max_row_blocks(row_bytes), want = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
   return want < most ? want : most;
 }
 
-// Workgroups of the shared walk that run at once.
-int walk_slots(int nr) {
+// The largest dynamic LDS a walk takes: the joins' 135 KiB, or the own walk's prefix of kMaxBatch rows.
+constexpr int kMaxLds = 150 * 1024;
+constexpr int kMaxBatch = 8192;
+
+int num_cus() {
   int dev = 0, cus = 0;
   if (hipGetDevice(&dev) != hipSuccess ||
       hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus < 1)
     cus = 256;
-  return nr == 4 ? cus : 2 * cus;
+  return cus;
 }
 
+constexpr int kSharedPerCU = 1;
+
 struct Plan {
-  int nr, chunks, segments;
-  int64_t rows() const { return 16 * nr; }
+  int nr, chunks, items, own_waves;
+  bool split;
 };
 
-// Row chunks and segments of a launch: as many segments as fill the workgroup slots once, and one
-// per group for the pieces that are not whole.
-Plan make_plan(bool fp8, int d, int n_groups, int64_t max_rows, int hkv, int g) {
+// Row chunks and items of a launch: kSharedPerCU shared workgroups per CU, at least one per group and
+// chunk (then nothing is cut).  The own
+// walk (own_sets > 0: the sets of pages it has at most) gets a wave per SIMD, two where a set is at most
+// 8 KiB, as the decode walk does.
+Plan make_plan(int row_bytes, bool small_sets, int n_groups, int64_t max_rows, int hkv, int g, int64_t own_sets,
+               int max_blocks) {
   Plan p;
-  const int64_t rows = max_rows * g;
-  p.nr = row_blocks(fp8, d, rows);
+  const int64_t rows = n_groups > 0 ? max_rows * g : 0;
+  p.nr = row_blocks(row_bytes, rows);
   p.chunks = (int)((rows + 16 * p.nr - 1) / (16 * p.nr));
-  const int64_t per = (int64_t)hkv * p.chunks;
-  const int64_t parts = walk_slots(p.nr) / (per > 0 ? per : 1);
-  p.segments = n_groups + (int)(parts > n_groups ? parts : 0);
+  const int64_t least = (int64_t)n_groups * p.chunks, most = num_cus() * kSharedPerCU / hkv;
+  p.split = p.chunks > 0 && most > least && most * max_blocks < 0x7fffffff;
+  p.items = p.split ? (int)most : least < 0x7fffffff ? (int)least : 0x7fffffff;
+  const int64_t waves = (int64_t)num_cus() * (small_sets ? 8 : 4), want = ((own_sets + 1) / 2 + 3) & ~3ll;
+  p.own_waves = (int)(want < waves ? want : waves);
   return p;
 }
 
-size_t plan_bytes(const Plan& p, int hkv, int d) {
-  return (size_t)p.segments * hkv * p.chunks * 16 * p.nr * (d + 2) * sizeof(float);
+// Workspace layout in floats: shared partials, own partials, the own walk's prefix.
+struct Layout {
+  size_t part_ml, own_acc, own_ml, own_pref, total;
+};
+Layout make_layout(const Plan& p, int n_rows, int hkv, int g, int d) {
+  Layout l;
+  const size_t rows = p.split || p.own_waves > 0 ? (size_t)p.items * hkv * 16 * p.nr : 0;
+  const size_t own = p.own_waves > 0 ? ((size_t)p.own_waves + (size_t)n_rows * hkv) * g : 0;
+  l.part_ml = rows * d;
+  l.own_acc = l.part_ml + rows * 2;
+  l.own_ml = l.own_acc + own * d;
+  l.own_pref = l.own_ml + own * 2;
+  l.total = l.own_pref + (p.own_waves > 0 ? (size_t)n_rows + 1 : 0);
+  return l;
 }
 
 template <int DT, int D, bool kFp8, int NR, bool NT>
-void launch_walk_n(const RowArgs& a, hipStream_t stream) {
-  constexpr int lds = (int)(join_floats<D, NR, kWaves>() * sizeof(float));
+void launch_walk_n(RowArgs a, hipStream_t stream) {
+  using S = Shape<DT, D, kFp8, NR>;
+  const int pref = a.own_waves > 0 ? (2 * a.n_rows + 1) * (int)sizeof(int32_t) : 0;
+  const int lds = a.shared_wgs > 0 && S::kLds > pref ? S::kLds : pref;
   static std::atomic<uint64_t> done{0};
-  allow_lds(reinterpret_cast<const void*>(&rows_walk_kernel<DT, D, kFp8, NR, NT>), lds, done);
-  const unsigned n = ((unsigned)(a.segments * a.Hkv) + 7) / 8 * 8 * (unsigned)a.chunks;
-  rows_walk_kernel<DT, D, kFp8, NR, NT><<<n, kThreads, lds, stream>>>(a, a.bt);
+  allow_lds(reinterpret_cast<const void*>(&rows_walk_kernel<DT, D, kFp8, NR, NT>), kMaxLds, done);
+  rows_walk_kernel<DT, D, kFp8, NR, NT><<<a.shared_wgs + a.own_waves / 4, 256, lds, stream>>>(a, a.bt);
 }
 
 template <int DT, int D, bool kFp8>
-void launch_walk_d(int nr, const RowArgs& a, hipStream_t stream) {
-  constexpr int most = max_row_blocks(kFp8, D);
+void launch_d(int nr, bool shared_chunks, RowArgs a, hipStream_t stream) {
+  constexpr int most = max_row_blocks(Shape<DT, D, kFp8, 1>::kRow);
+  a.unit = 4 * PageOps<DT, D, kFp8>::kPages;
+  a.shared_wgs = a.items * a.Hkv;
   // One chunk reads every page once: streaming loads.  Several share them through the L2.
-  if (nr == most && a.chunks > 1) return launch_walk_n<DT, D, kFp8, most, false>(a, stream);
-  if constexpr (most >= 4) {
-    if (nr == 4) return launch_walk_n<DT, D, kFp8, 4, true>(a, stream);
+  if (a.shared_wgs + a.own_waves == 0) {
+    // nothing to walk: the join writes zeros
+  } else if (nr == most && shared_chunks) {
+    launch_walk_n<DT, D, kFp8, most, false>(a, stream);
+  } else if (nr == 1) {
+    launch_walk_n<DT, D, kFp8, 1, true>(a, stream);
+  } else if constexpr (most >= 2) {
+    if (nr == 2) launch_walk_n<DT, D, kFp8, 2, true>(a, stream);
+    else launch_walk_n<DT, D, kFp8, most, true>(a, stream);
   }
-  if constexpr (most >= 2) {
-    if (nr == 2) return launch_walk_n<DT, D, kFp8, 2, true>(a, stream);
-  }
-  launch_walk_n<DT, D, kFp8, 1, true>(a, stream);
-}
-
-template <int DT, int D, bool kFp8, int W>
-void launch_own_w(const RowArgs& a, int batch, hipStream_t stream) {
-  constexpr int lds = (int)(join_floats<D, 1, W>() * sizeof(float));
-  static std::atomic<uint64_t> done{0};
-  allow_lds(reinterpret_cast<const void*>(&prefix_own_kernel<DT, D, kFp8, W>), lds, done);
-  const unsigned n = (unsigned)batch * a.Hkv * ((a.G + 15) / 16);
-  prefix_own_kernel<DT, D, kFp8, W><<<n, 64 * W, lds, stream>>>(a, a.bt);
-}
-
-template <int DT, int D, bool kFp8>
-void launch_d(int nr, const RowArgs& a, hipStream_t stream) {
-  if (a.n_groups > 0 && a.chunks > 0) launch_walk_d<DT, D, kFp8>(nr, a, stream);
-  if (a.prefix) {
-    launch_own_w<DT, D, kFp8, 4>(a, a.n_rows, stream);
-  } else if (a.segments > a.n_groups) {
-    rows_merge_kernel<DT, D><<<(unsigned)a.n_rows * a.Hkv, kThreads, 0, stream>>>(a);
-  }
+  if (a.prefix || a.split)
+    rows_join_kernel<DT, D><<<(unsigned)a.n_rows * a.Hkv, 256, 0, stream>>>(a);
 }
 
 template <int DT, bool kFp8>
-void launch_t(int head_dim, int nr, const RowArgs& a, hipStream_t stream) {
+void launch_t(int head_dim, int nr, bool shared_chunks, const RowArgs& a, hipStream_t stream) {
   switch (head_dim) {
-    case 64: launch_d<DT, 64, kFp8>(nr, a, stream); break;
-    case 128: launch_d<DT, 128, kFp8>(nr, a, stream); break;
-    default: launch_d<DT, 256, kFp8>(nr, a, stream); break;
+    case 64: launch_d<DT, 64, kFp8>(nr, shared_chunks, a, stream); break;
+    case 128: launch_d<DT, 128, kFp8>(nr, shared_chunks, a, stream); break;
+    default: launch_d<DT, 256, kFp8>(nr, shared_chunks, a, stream); break;
   }
 }
 
-void launch(int dtype, bool fp8, int head_dim, int nr, const RowArgs& a, hipStream_t stream) {
+void launch(int dtype, bool fp8, int head_dim, int nr, bool shared_chunks, const RowArgs& a, hipStream_t stream) {
   if (fp8) {
-    if (dtype == IVAKV_F16) launch_t<IVAKV_F16, true>(head_dim, nr, a, stream);
-    else launch_t<IVAKV_BF16, true>(head_dim, nr, a, stream);
+    if (dtype == IVAKV_F16) launch_t<IVAKV_F16, true>(head_dim, nr, shared_chunks, a, stream);
+    else launch_t<IVAKV_BF16, true>(head_dim, nr, shared_chunks, a, stream);
     return;
   }
   switch (dtype) {
-    case IVAKV_F16: launch_t<IVAKV_F16, false>(head_dim, nr, a, stream); break;
-    case IVAKV_BF16: launch_t<IVAKV_BF16, false>(head_dim, nr, a, stream); break;
-    default: launch_t<IVAKV_F32, false>(head_dim, nr, a, stream); break;
+    case IVAKV_F16: launch_t<IVAKV_F16, false>(head_dim, nr, shared_chunks, a, stream); break;
+    case IVAKV_BF16: launch_t<IVAKV_BF16, false>(head_dim, nr, shared_chunks, a, stream); break;
+    default: launch_t<IVAKV_F32, false>(head_dim, nr, shared_chunks, a, stream); break;
   }
 }
 
@@ -1001,9 +1172,17 @@ int check_geometry(const char* name, int n_groups, int num_q_heads, int num_kv_h
   return IVAKV_OK;
 }
 
+Plan plan_of(int n_groups, int n_rows, int num_q_heads, int num_kv_heads, int head_dim, int max_rows, int dtype,
+             int max_blocks, bool prefix) {
+  const int row_bytes = head_dim * dtype_size(dtype);
+  // (FP8 pages hold half the bytes of the queries' type: they are not told apart here, so that
+  // the workspace does not depend on the pages)
+  return make_plan(row_bytes, row_bytes <= 256, n_groups, max_rows, num_kv_heads, num_q_heads / num_kv_heads,
+                   prefix ? (int64_t)n_rows * num_kv_heads * max_blocks : 0, max_blocks);
+}
+
 int check_plan(const char* name, const Plan& p, int num_kv_heads) {
-  if ((int64_t)(p.segments + 8) * num_kv_heads > 0x7fffffff ||
-      ((int64_t)p.segments * num_kv_heads + 8) * p.chunks > 0x7fffffff)
+  if ((int64_t)p.items * num_kv_heads > 0x3fffffff)
     return fail(IVAKV_E_SHAPE, "%s: launch too large", name);
   return IVAKV_OK;
 }
@@ -1030,38 +1209,49 @@ int rows_entry(const char* name, RowArgs a, int batch, int num_q_heads, int head
     return fail(IVAKV_E_ARG, "%s: k_scale / v_scale must be 16-byte aligned device pointers", name);
   if (!(scale == scale)) return fail(IVAKV_E_ARG, "%s: scale is NaN", name);
   a.G = num_q_heads / a.Hkv;
-  if ((int64_t)a.n_rows * num_q_heads > 0x7fffffff) return fail(IVAKV_E_SHAPE, "%s: launch too large", name);
+  if ((int64_t)a.n_rows * num_q_heads > 0x7fffffff)
+    return fail(IVAKV_E_SHAPE, "%s: launch too large", name);
+  if (a.prefix && (a.n_rows > kMaxBatch || (int64_t)a.n_rows * a.max_blocks > 0x7fffffff / a.Hkv))
+    return fail(IVAKV_E_SHAPE, "%s: at most %d rows, and rows x max_blocks x num_kv_heads below 2^31 (got %d, %d, %d)",
+                name, kMaxBatch, a.n_rows, a.max_blocks, a.Hkv);
   a.max_rows = a.max_rows < a.n_rows ? a.max_rows : a.n_rows;
-  const Plan p = make_plan(fp8, head_dim, a.n_groups, a.max_rows, a.Hkv, a.G);
+  const Plan p = plan_of(a.n_groups, a.n_rows, num_q_heads, a.Hkv, head_dim, a.max_rows, dtype, a.max_blocks,
+                         a.prefix);
   const int bad = check_plan(name, p, a.Hkv);
   if (bad != IVAKV_OK) return bad;
-  const size_t need = plan_bytes(p, a.Hkv, head_dim);
+  const Layout l = make_layout(p, a.n_rows, a.Hkv, a.G, head_dim);
+  const size_t need = l.total * sizeof(float);
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
     return fail(IVAKV_E_WORKSPACE, "%s: workspace of %zu bytes (16-byte aligned) required, got %zu", name, need,
                 workspace ? workspace_bytes : (size_t)0);
-  a.chunks = p.chunks;
-  a.rows_chunk = 16 * p.nr;
-  a.segments = p.segments;
+  a.rows_shift = p.nr == 1 ? 4 : p.nr == 2 ? 5 : 6;
+  a.items = p.items;
+  a.split = p.split;
+  a.own_waves = p.own_waves;
   a.part_acc = static_cast<float*>(workspace);
-  a.part_ml = a.part_acc + (size_t)p.segments * a.Hkv * p.chunks * 16 * p.nr * head_dim;
+  a.part_ml = a.part_acc + l.part_ml;
+  a.own_acc = a.part_acc + l.own_acc;
+  a.own_ml = a.part_acc + l.own_ml;
+  a.own_pref = reinterpret_cast<int32_t*>(a.part_acc + l.own_pref);
   a.scale_log2 = (float)((double)scale * 1.4426950408889634);
   a.window = a.window > 0 ? a.window : 0;
-  launch(dtype, fp8, head_dim, p.nr, a, stream);
+  launch(dtype, fp8, head_dim, p.nr, p.chunks > 1, a, stream);
   return launch_status(name);
 }
 
 int workspace_size(const char* name, int n_groups, int n_rows, int num_q_heads, int num_kv_heads, int head_dim,
-                   int max_rows, int dtype, int fp8, size_t* bytes) {
+                   int max_rows, int dtype, int max_blocks, bool prefix, size_t* bytes) {
   if (!bytes) return fail(IVAKV_E_ARG, "%s: null bytes", name);
   *bytes = 0;
   const int err = check_geometry(name, n_groups, num_q_heads, num_kv_heads, head_dim, max_rows, dtype);
   if (err != IVAKV_OK) return err;
-  if (n_rows < 0) return fail(IVAKV_E_ARG, "%s: negative row count", name);
-  const Plan p = make_plan(fp8 != 0, head_dim, n_groups, max_rows < n_rows ? max_rows : n_rows, num_kv_heads,
-                           num_q_heads / num_kv_heads);
+  if (n_rows < 0 || max_blocks < 0)
+    return fail(IVAKV_E_ARG, "%s: bad sizes rows=%d max_blocks=%d", name, n_rows, max_blocks);
+  const Plan p = plan_of(n_groups, n_rows, num_q_heads, num_kv_heads, head_dim,
+                         max_rows < n_rows ? max_rows : n_rows, dtype, max_blocks, prefix);
   const int bad = check_plan(name, p, num_kv_heads);
   if (bad != IVAKV_OK) return bad;
-  *bytes = plan_bytes(p, num_kv_heads, head_dim);
+  *bytes = make_layout(p, n_rows, num_kv_heads, num_q_heads / num_kv_heads, head_dim).total * sizeof(float);
   return IVAKV_OK;
 }
 
@@ -1071,10 +1261,10 @@ int workspace_size(const char* name, int n_groups, int n_rows, int num_q_heads, 
 using namespace ivakv;
 
 extern "C" int ivakv_prefix_workspace_size(int batch, int n_groups, int max_group, int num_q_heads,
-                                           int num_kv_heads, int head_dim, int dtype, int fp8,
+                                           int num_kv_heads, int head_dim, int max_blocks, int dtype,
                                            size_t* bytes) {
   return workspace_size("ivakv_prefix_workspace_size", n_groups, batch, num_q_heads, num_kv_heads, head_dim,
-                        max_group, dtype, fp8, bytes);
+                        max_group, dtype, max_blocks, true, bytes);
 }
 
 extern "C" int ivakv_prefix_decode_attn(const void* q, const void* k_pool, const void* v_pool,
@@ -1110,10 +1300,10 @@ extern "C" int ivakv_prefix_decode_attn(const void* q, const void* k_pool, const
 }
 
 extern "C" int ivakv_cross_workspace_size(int batch, int n_tok, int max_query_len, int num_q_heads,
-                                          int num_kv_heads, int head_dim, int dtype, int fp8,
-                                           size_t* bytes) {
+                                          int num_kv_heads, int head_dim, int max_blocks, int dtype,
+                                          size_t* bytes) {
   return workspace_size("ivakv_cross_workspace_size", batch, n_tok, num_q_heads, num_kv_heads, head_dim,
-                        max_query_len, dtype, fp8, bytes);
+                        max_query_len, dtype, max_blocks, false, bytes);
 }
 
 extern "C" int ivakv_cross_attn(const void* q, const void* k_pool, const void* v_pool, const float* k_scale,

@@ -766,13 +766,13 @@ def _row_workspace_bytes(entry: str, *geometry: int) -> int:
 
 
 def cross_workspace_bytes(batch: int, n_tok: int, max_query_len: int, num_q_heads: int,
-                          num_kv_heads: int, head_dim: int, dtype: torch.dtype,
-                          fp8: bool = False) -> int:
-    """Workspace bytes of :func:`paged_cross_attention` (``dtype`` of the queries, ``fp8``: FP8
-    pools).  The workspace needs no initialisation."""
+                          num_kv_heads: int, head_dim: int, max_blocks: int,
+                          dtype: torch.dtype) -> int:
+    """Workspace bytes of :func:`paged_cross_attention` (``dtype`` of the queries).  The workspace
+    needs no initialisation."""
     return _row_workspace_bytes("ivakv_cross_workspace_size", int(batch), int(n_tok),
                                 int(max_query_len), int(num_q_heads), int(num_kv_heads),
-                                int(head_dim), dtype_code(dtype), int(fp8))
+                                int(head_dim), int(max_blocks), dtype_code(dtype))
 
 
 def paged_cross_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
@@ -807,7 +807,7 @@ def paged_cross_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.T
     if scale is None:
         scale = 1.0 / math.sqrt(head_dim)
     workspace = _sized_workspace(workspace, dev, cross_workspace_bytes(
-        batch, n_tok, max_query_len, hq, hkv, head_dim, q.dtype, scales[0] is not None))
+        batch, n_tok, max_query_len, hq, hkv, head_dim, block_tables.shape[1], q.dtype))
     _abi.call("ivakv_cross_attn", q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), *scales,
               block_tables.data_ptr(), context_lens.data_ptr(), query_start.data_ptr(), n_tok,
               out.data_ptr(), workspace.data_ptr(), workspace.numel() * workspace.element_size(),
@@ -817,13 +817,13 @@ def paged_cross_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.T
 
 
 def prefix_workspace_bytes(batch: int, n_groups: int, max_group: int, num_q_heads: int,
-                           num_kv_heads: int, head_dim: int, dtype: torch.dtype,
-                           fp8: bool = False) -> int:
-    """Workspace bytes of :func:`paged_prefix_decode_attention` (``dtype`` of the queries,
-    ``fp8``: FP8 pools).  The workspace needs no initialisation."""
+                           num_kv_heads: int, head_dim: int, max_blocks: int,
+                           dtype: torch.dtype) -> int:
+    """Workspace bytes of :func:`paged_prefix_decode_attention` (``dtype`` of the queries).  The
+    workspace needs no initialisation."""
     return _row_workspace_bytes("ivakv_prefix_workspace_size", int(batch), int(n_groups),
                                 int(max_group), int(num_q_heads), int(num_kv_heads),
-                                int(head_dim), dtype_code(dtype), int(fp8))
+                                int(head_dim), int(max_blocks), dtype_code(dtype))
 
 
 def paged_prefix_decode_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
@@ -840,12 +840,13 @@ def paged_prefix_decode_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool:
 
     Rows ``group_start[g] .. group_start[g+1]-1`` (int32 ``[n_groups+1]``, rising) form group g, and
     their block-table rows have to agree in the full pages of the group's first ``prefix_lens[g]``
-    tokens (int32 ``[n_groups]``); those are read from the table of the first row that is as long.
-    Rows of no group, and rows shorter than their group's prefix, read all of their own pages.  Same result as
-    :func:`paged_decode_attention` within the attention tolerance.  ``max_group`` (>= the largest
-    group's rows) sizes the launch; when omitted it is read back from ``group_start`` (a device
-    sync), which is then checked.  ``workspace`` (:func:`prefix_workspace_bytes`) is kept per device
-    and stream when omitted.
+    tokens (int32 ``[n_groups]``); those are read from the table of the first row that takes part.  A
+    row takes part if it has the whole prefix and its window cuts nothing off; any other, and rows of
+    no group, read all of their visible pages.  Same result as :func:`paged_decode_attention` within
+    the attention tolerance.  ``max_group`` (>= the largest group's rows) sizes the launch; when
+    omitted it is read back from ``group_start`` (a device sync), which is then checked.
+    ``workspace`` (:func:`prefix_workspace_bytes`) is kept per device and stream when omitted.  At
+    most 8192 rows.
 
     Replaces the cache branch of ``AttentionTorch.forward`` (src/core/attention.py:77-102).
     """
@@ -865,7 +866,7 @@ def paged_prefix_decode_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool:
     if scale is None:
         scale = 1.0 / math.sqrt(head_dim)
     workspace = _sized_workspace(workspace, dev, prefix_workspace_bytes(
-        batch, n_groups, max_group, hq, hkv, head_dim, q.dtype, scales[0] is not None))
+        batch, n_groups, max_group, hq, hkv, head_dim, block_tables.shape[1], q.dtype))
     _abi.call("ivakv_prefix_decode_attn", q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), *scales,
               block_tables.data_ptr(), context_lens.data_ptr(), group_start.data_ptr(),
               prefix_lens.data_ptr(), n_groups, out.data_ptr(), workspace.data_ptr(),

@@ -42,7 +42,8 @@ def test_row_entry_refusals(iva, name, build):
             (dict(ks=FAKE), a.E_ARG), (dict(ks=FAKE, vs=FAKE + 4), a.E_ARG), (dict(scale=float("nan")), a.E_ARG),
             (dict(ws=None), a.E_WORKSPACE), (dict(ws_bytes=64), a.E_WORKSPACE), (dict(ws=FAKE + 4), a.E_WORKSPACE),
             (dict(hq=1 << 30, hkv=1 << 30, n_tok=1 << 20) if name == "ivakv_cross_attn" else
-             dict(hq=1 << 30, hkv=1 << 30, batch=1 << 20), a.E_SHAPE)]:
+             dict(hq=1 << 30, hkv=1 << 30, batch=1 << 20), a.E_SHAPE),
+            *([] if name == "ivakv_cross_attn" else [(dict(batch=8193), a.E_SHAPE), (dict(max_blocks=1 << 30), a.E_SHAPE)])]:
         assert call(iva, name, *build(iva, **over)) == status, over
         assert name in a.last_error()
 
@@ -63,14 +64,16 @@ def test_row_workspace_sizes(iva):
     a = iva._abi
     n = ctypes.c_size_t(7)
     for name in ("ivakv_cross_workspace_size", "ivakv_prefix_workspace_size"):
-        assert call(iva, name, 2, 8, 4, 8, 2, 100, a.F16, 0, ctypes.byref(n)) == a.E_SHAPE and n.value == 0
-        assert call(iva, name, 2, 8, 4, 8, 2, 128, 9, 0, ctypes.byref(n)) == a.E_DTYPE
-        assert call(iva, name, 2, 8, 4, 8, 2, 128, a.F16, 0, None) == a.E_ARG
-        assert call(iva, name, 2, 8, 4, 8, 3, 128, a.F16, 0, ctypes.byref(n)) == a.E_SHAPE
+        assert call(iva, name, 2, 8, 4, 8, 2, 100, 9, a.F16, ctypes.byref(n)) == a.E_SHAPE and n.value == 0
+        assert call(iva, name, 2, 8, 4, 8, 2, 128, 9, 9, ctypes.byref(n)) == a.E_DTYPE
+        assert call(iva, name, 2, 8, 4, 8, 2, 128, 9, a.F16, None) == a.E_ARG
+        assert call(iva, name, 2, 8, 4, 8, 3, 128, 9, a.F16, ctypes.byref(n)) == a.E_SHAPE
+    assert call(iva, "ivakv_prefix_workspace_size", 2, 1, 2, 8, 2, 128, -1, a.F16, ctypes.byref(n)) == a.E_ARG
     # grows with nothing but the launch: no rows, no partials
-    assert iva.cross_workspace_bytes(0, 0, 0, 8, 2, 128, torch.float16) == 0
-    assert iva.prefix_workspace_bytes(4, 0, 0, 8, 2, 128, torch.float16) == 0
-    assert iva.prefix_workspace_bytes(64, 1, 64, 32, 8, 128, torch.float16) % 16 == 0
+    assert iva.cross_workspace_bytes(0, 0, 0, 8, 2, 128, 100, torch.float16) == 0
+    assert iva.prefix_workspace_bytes(0, 0, 0, 8, 2, 128, 100, torch.float16) == 0
+    wide, narrow = (iva.prefix_workspace_bytes(64, 1, 64, 32, 8, 128, n, torch.float16) for n in (1000, 1))
+    assert wide > narrow > 0
 
 
 def pools(iva, dtype=torch.float16):

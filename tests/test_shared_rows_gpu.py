@@ -362,7 +362,7 @@ def test_row_ops_device_refusals(iva, dev):
     with pytest.raises(ValueError, match="query_start must rise"):
         cross(iva, dev, x)
     x.qs = torch.tensor([0, 2, 4], dtype=torch.int32)
-    n = iva.cross_workspace_bytes(2, 4, 2, 8, 2, 64, torch.float16)
+    n = iva.cross_workspace_bytes(2, 4, 2, 8, 2, 64, x.bt.shape[1], torch.float16)
     ws = torch.full((n + 256,), 0x7F, dtype=torch.uint8, device=dev)
     x.check(cross(iva, dev, x, workspace=ws[:n], max_query_len=2), cross_ref(x), "own workspace")
     assert (ws[n:] == 0x7F).all()
