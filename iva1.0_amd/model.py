@@ -44,7 +44,7 @@ from __future__ import annotations
 
 import math
 from dataclasses import dataclass
-from typing import Any, Dict, Optional, Tuple
+from typing import Any, Dict, List, Optional, Tuple
 
 import torch
 import torch.autograd.forward_ad as fwAD
@@ -53,8 +53,9 @@ import torch.nn.functional as F
 from torch.nn.modules.module import _has_any_global_hook
 
 from .ops import (FP8, LINEAR_MAX_ROWS, LINEAR_NORM_MAX_K, LINEAR_NORM_MAX_ROWS, NORM_MAX_D,
-                  block_decode, kv_gather, linear_rows, paged_decode_append_attention,
-                  paged_prefill_attention, rms_norm, rope_, swiglu)
+                  TokenLogprobs, block_decode, kv_append, kv_gather, linear_rows, paged_cross_attention,
+                  paged_decode_append_attention, paged_prefill_attention,
+                  paged_prefix_decode_attention, rms_norm, rope_, swiglu, token_logprobs)
 from .paged_cache import OwnPages, PagedKVCache
 
 
@@ -193,6 +194,15 @@ class LayeredKVCache:
     def commit(self, t: int) -> None:
         if self._cursor == 0:
             self.seq_len += t
+
+    def fork(self, samples: int) -> None:
+        """PagedKVCache.fork on contiguous caches: every sequence's rows repeated."""
+        if self._cursor:
+            raise RuntimeError("a forward is in progress on this cache")
+        for c in self.layers:
+            c.k, c.v = (t.repeat_interleave(int(samples), dim=0) for t in (c.k, c.v))
+            c.batch_size *= int(samples)
+        self.batch_size *= int(samples)
 
 
 # ------------------------------------------------------------- layer kernels
@@ -463,6 +473,22 @@ class AttentionTorch(_AttentionBase):
         return self.o_proj(out), kv_cache
 
 
+# Bytes of K and V per layer that forked sequences would read again, from which a decode step
+# appends and attends through the shared prefix instead of in the one fused step.
+SHARED_MIN_BYTES = 32 << 20
+
+
+def _reads_shared(cache: Any, window: Optional[int]) -> bool:
+    """A paged cache whose forked sequences share enough for paged_prefix_decode_attention, and
+    see all of it."""
+    shared = getattr(cache, "shared", None)
+    if shared is None or (window and 0 < window <= cache.seq_len):
+        return False
+    pool = cache.pool
+    row = 2 * pool.num_kv_heads * pool.head_dim * pool.dtype.itemsize
+    return shared.saved_tokens * row >= SHARED_MIN_BYTES
+
+
 class PagedAttention(_AttentionBase):
     """``attn_impl="hip_paged"``: the attention module on a PagedKVCache.
 
@@ -475,9 +501,10 @@ class PagedAttention(_AttentionBase):
     A contiguous ``KVCache`` is taken over as a PagedKVCache (:meth:`_adopt`), which is
     returned in its place.  Without a cache a causal step runs the same kernels on a
     one-layer paged cache of its own tokens, and None is returned, as the reference
-    returns (attention.py:74-75).  Non-causal attention (``config.causal`` False) is
-    evaluated in torch on the gathered pages: the paged kernels are causal.  With a
-    sliding window, once the forward's last layer is enqueued the cache releases the
+    returns (attention.py:74-75).  Non-causal attention (``config.causal`` False) runs
+    ivakv_cross_attn over the pages at inference on 16-bit tensors, and torch on the gathered
+    pages otherwise.  Decode steps of sequences forked from one prompt (PagedKVCache.fork) read the
+    pages they share once (ivakv_prefix_decode_attn) where that pays.  With a sliding window, once the forward's last layer is enqueued the cache releases the
     pages no later query can see (:meth:`PagedKVCache.release_window`; the sink pages
     stay resident), so a long sequence holds about window + sinks tokens per layer.
     A padding mask (``attention_mask`` with zeros, src/core/attention.py:95-97) is applied
@@ -504,11 +531,12 @@ class PagedAttention(_AttentionBase):
                 return self._split_heads(linear_rows(x, w))
         return super()._project(x)
 
-    def _decodes(self, x, attention_mask, cache) -> bool:
+    def _decodes(self, x, attention_mask, cache, window=None) -> bool:
         """A decode step that block_decode runs whole: one token per sequence onto a plain
         paged cache of 16-bit pages like x or FP8 pages, causal, without mask or RoPE."""
         if (attention_mask is not None or type(cache) is not PagedKVCache or x.shape[1] != 1
-                or not self.causal or self.rope or (self.training and self.dropout > 0)):
+                or not self.causal or self.rope or (self.training and self.dropout > 0)
+                or _reads_shared(cache, window)):
             return False
         pool = cache.pool
         return ((pool.dtype is x.dtype or pool.fp8) and pool.num_kv_heads == self.n_kv_heads
@@ -545,7 +573,9 @@ class PagedAttention(_AttentionBase):
         key_ok = self._key_mask(attention_mask)
         b, s, _ = x.shape
         returned = kv_cache
-        if kv_cache is None and self.causal:
+        cross = (not self.causal and key_ok is None and not (sliding_window and sliding_window > 0)
+                 and _plain_type(x) and _plain_mode() and b * s)
+        if kv_cache is None and (self.causal or cross):
             if x.is_cuda and b * s:
                 kv_cache = OwnPages(b, s, self.n_kv_heads, self.head_dim, x.device, x.dtype)
             else:
@@ -578,10 +608,23 @@ class PagedAttention(_AttentionBase):
             # (ivakv_gather) by the kernels, and the masked attention evaluated on the
             # gathered keys in torch (the paged attention kernels take no per-key mask)
             decode = s == 1 and self.causal and key_ok is None
+            shared_prefix = decode and _reads_shared(kv_cache, window)
             fp8 = kv_cache.pool.fp8
             view = kv_cache.layer_step(k.contiguous(), v.contiguous(), append=not decode,
                                        rope_positions=rope_pos, rope_theta=self.rope_theta)
-            if decode:
+            if decode and shared_prefix:
+                # sequences forked from one prompt: the rows are appended, then the pages that
+                # the sequences share are read once for all of them (ivakv_prefix_decode_attn)
+                shared = view.shared
+                kv_append(k.view(b, self.n_kv_heads, self.head_dim), v.view(b, self.n_kv_heads, self.head_dim),
+                          view.k_pool, view.v_pool, view.slot_mapping, **view.scales)
+                o = paged_prefix_decode_attention(
+                    q.view(b, self.n_heads, self.head_dim), view.k_pool, view.v_pool, view.block_tables,
+                    view.context_lens, shared.group_start, shared.prefix_lens, scale=self.scale,
+                    window=window or 0, n_sink=n_sink if window else 0, max_group=shared.max_group,
+                    **view.scales)
+                out = o.view(b, 1, self.n_heads, self.head_dim)
+            elif decode:
                 # append + attend in one op: the new row lands at position L-1 of each page
                 # table and is scored straight from k / v (ivakv_decode_append_attn; on
                 # FP8 pages quantized as the append would, ivakv_decode_append_attn_fp8)
@@ -602,8 +645,16 @@ class PagedAttention(_AttentionBase):
                     window=window or 0, n_sink=n_sink if window else 0, max_query_len=s,
                     **view.scales)
                 out = o.view(b, s, self.n_heads, self.head_dim)
+            elif cross and _plain_type(q):
+                # non-causal: every row over all of its sequence's keys (ivakv_cross_attn)
+                qs = torch.arange(0, (b + 1) * s, s, dtype=torch.int32, device=x.device)
+                o = paged_cross_attention(
+                    q.reshape(b * s, self.n_heads, self.head_dim), view.k_pool, view.v_pool,
+                    view.block_tables, view.context_lens, qs, scale=self.scale, max_query_len=s,
+                    **view.scales)
+                out = o.view(b, s, self.n_heads, self.head_dim)
             else:
-                # non-causal, a padding mask, or fp32 queries on FP8 pages: gather
+                # a padding mask, fp32 queries on FP8 pages, or non-causal under autograd: gather
                 # (dequantized for FP8) and evaluate the masked attention of the new
                 # tokens in torch
                 total = view.start + s
@@ -805,7 +856,7 @@ class TransformerBlock(nn.Module):
             wo = _linear_weight(attn._modules["o_proj"], x, d, attn.n_heads * attn.head_dim)
             if (qkv is not None and wo is not None and w is not None and w[2].shape[0] == d
                     and _rows(x) <= _block_rows(d, w[0].shape[0])):
-                if attn._decodes(x, attention_mask, kv_cache):
+                if attn._decodes(x, attention_mask, kv_cache, sliding_window):
                     return self._decode_step(x, qkv, wo, w, kv_cache, sliding_window, sink_cfg)
                 in_norm = (x.numel() <= LINEAR_NORM_MAX_ROWS * x.shape[-1]
                            and x.shape[-1] <= LINEAR_NORM_MAX_K)
@@ -834,6 +885,39 @@ class TransformerBlock(nn.Module):
         return x + ffn(y), cache
 
 
+def _logprobs_of(logits: torch.Tensor, tokens: torch.Tensor, top_k: int) -> TokenLogprobs:
+    """:func:`token_logprobs`, or its formula in torch for logits that are not on a GPU."""
+    if logits.is_cuda:
+        return token_logprobs(logits, tokens, top_k)
+    logp = torch.log_softmax(logits.float(), dim=-1)
+    given = (tokens >= 0) & (tokens < logits.shape[-1])
+    picked = logp.gather(-1, torch.where(given, tokens, 0)[..., None].long())[..., 0]
+    order = torch.sort(logits, dim=-1, descending=True, stable=True).indices[..., :top_k]
+    entropy = -torch.where(logp > float("-inf"), logp.exp() * logp, torch.zeros_like(logp)).sum(dim=-1)
+    return TokenLogprobs(torch.where(given, picked, torch.zeros_like(picked)), entropy,
+                         logp.gather(-1, order), order)
+
+
+class _Recorder:
+    """The log probabilities of generated tokens, a step at a time."""
+
+    def __init__(self, top_k: int):
+        self.top_k = top_k
+        self.steps: List[Any] = []
+
+    def of(self, logits: torch.Tensor, tok: torch.Tensor) -> List[torch.Tensor]:
+        return list(_logprobs_of(logits, tok[:, 0], self.top_k))
+
+    def keep(self, found: List[torch.Tensor]) -> None:
+        self.steps.append(found)
+
+    def add(self, logits: torch.Tensor, tok: torch.Tensor) -> None:
+        self.keep(self.of(logits, tok))
+
+    def result(self) -> TokenLogprobs:
+        return TokenLogprobs(*(torch.stack(t, dim=1) for t in zip(*self.steps)))
+
+
 class Transformer(nn.Module):
     """src/core/transformer.py:154-320 at its interfaces."""
 
@@ -859,9 +943,11 @@ class Transformer(nn.Module):
         elif isinstance(module, nn.Embedding):
             torch.nn.init.normal_(module.weight, mean=0.0, std=0.02)
 
-    def new_kv_cache(self, batch_size: int, max_seq_len: int, device=None, dtype=None):
+    def new_kv_cache(self, batch_size: int, max_seq_len: int, device=None, dtype=None,
+                     samples: int = 1, prompt_len: int = 0):
         """An empty cache of the configured backend for ``batch_size`` sequences of up to
-        ``max_seq_len`` tokens, one set of K/V per layer."""
+        ``max_seq_len`` tokens, one set of K/V per layer.  ``samples``: room to fork every
+        sequence into that many once it holds ``prompt_len`` tokens."""
         cfg = self.config
         device = device or self.token_embedding.weight.device
         dtype = dtype or self.token_embedding.weight.dtype
@@ -869,10 +955,14 @@ class Transformer(nn.Module):
         head_dim = cfg.d_model // cfg.n_heads
         if cfg.attn_impl == "hip_paged":
             page_dtype = FP8 if _cfg(cfg, "kv_cache_dtype", None) == "fp8" else dtype
+            bs, num_pages = _cfg(cfg, "kv_block_size", 16), _cfg(cfg, "kv_num_pages", None)
+            if num_pages is None and samples > 1:
+                per_seq = max(-(-max_seq_len // bs), 1)
+                num_pages = batch_size * (per_seq + (samples - 1) * (per_seq - prompt_len // bs))
             cache = PagedKVCache(batch_size, n_kv, head_dim, 0, device, page_dtype,
-                                 num_layers=cfg.n_layers, block_size=_cfg(cfg, "kv_block_size", 16),
-                                 max_seq_len=max_seq_len, num_pages=_cfg(cfg, "kv_num_pages", None),
-                                 compute_dtype=dtype)
+                                 num_layers=cfg.n_layers, block_size=bs,
+                                 max_seq_len=max_seq_len, num_pages=num_pages,
+                                 compute_dtype=dtype, max_seqs=batch_size * samples)
             cache.resize(max_seq_len)
             return cache
         return LayeredKVCache(batch_size, n_kv, head_dim, cfg.n_layers, device, dtype)
@@ -913,6 +1003,16 @@ class Transformer(nn.Module):
             outputs["value"] = self.value_head(x)
         return outputs
 
+    def score(self, input_ids: torch.Tensor, top_k: int = 0, **kwargs) -> TokenLogprobs:
+        """Log probabilities of ``input_ids[:, 1:]``, each given the tokens before it, with the
+        entropy (and the ``top_k`` likeliest tokens) at each of those positions: ``[B, S-1]``
+        results of :func:`token_logprobs` on one forward's logits, differentiable where the
+        backend is.  Keyword arguments go to :meth:`forward`."""
+        logits = self.forward(input_ids, **kwargs)["logits"]
+        # (whole rows of the logits, the last position with no token: nothing is copied)
+        tokens = F.pad(input_ids[:, 1:], (0, 1), value=-1)
+        return TokenLogprobs(*(t[:, :-1] for t in _logprobs_of(logits, tokens, top_k)))
+
     @torch.no_grad()
     def generate(self, input_ids: torch.Tensor, max_length: int = 100, temperature: float = 1.0,
                  top_p: float = 0.9, top_k: int = 50, do_sample: bool = True,
@@ -925,40 +1025,60 @@ class Transformer(nn.Module):
         reserved up front and its per-step bookkeeping runs on the device.  EOS
         stopping (``eos_token_id``) needs a host read per step; pass None to run
         all ``max_length`` steps without one.
+
+        ``num_samples=n`` (keyword) draws n continuations of every prompt, rows ``b * n ..
+        (b + 1) * n - 1`` of the result: the prompt runs once and its cache is forked
+        (:meth:`PagedKVCache.fork`).  ``return_logprobs=True`` returns ``(tokens, logprobs)``, a
+        :class:`TokenLogprobs` ``[rows, new tokens]`` of the generated tokens under the model's
+        own distribution (before temperature and filters), with ``top_logprobs=k`` likeliest
+        tokens at each position.
         """
         self.eval()
         batch_size, prompt_len = input_ids.shape
+        samples = int(kwargs.get("num_samples", 1))
+        if samples < 1:
+            raise ValueError(f"num_samples must be >= 1, got {samples}")
+        record = _Recorder(int(kwargs.get("top_logprobs", 0))) if kwargs.get("return_logprobs") else None
         own_cache = kwargs.get("kv_cache") is None
-        cache = kwargs.get("kv_cache") or self.new_kv_cache(batch_size, prompt_len + max_length)
+        cache = kwargs.get("kv_cache") or self.new_kv_cache(batch_size, prompt_len + max_length,
+                                                            samples=samples, prompt_len=prompt_len)
         use_graph = bool(kwargs.get("use_graph", False))
         if use_graph and not isinstance(cache, PagedKVCache):
             raise ValueError("use_graph needs attn_impl='hip_paged'")
-        out = torch.empty(batch_size, prompt_len + max_length, dtype=input_ids.dtype,
+        out = torch.empty(batch_size * samples, prompt_len + max_length, dtype=input_ids.dtype,
                           device=input_ids.device)
-        out[:, :prompt_len] = input_ids
+        out[:, :prompt_len] = input_ids.repeat_interleave(samples, dim=0)
         n = 0
         try:
             logits = self.forward(input_ids, kv_cache=cache)["logits"][:, -1, :]
+            if samples > 1:
+                cache.fork(samples)
+                logits = logits.repeat_interleave(samples, dim=0)
             tok = self._sample(logits, temperature, top_p, top_k, do_sample)
+            if record is not None:
+                record.add(logits, tok)
             out[:, prompt_len] = tok[:, 0]
             n = 1
             if use_graph and max_length > 1:
                 n = self._decode_graph(cache, tok, out, prompt_len, max_length, temperature,
-                                       top_p, top_k, do_sample)
+                                       top_p, top_k, do_sample, record)
             else:
                 while n < max_length and not (eos_token_id is not None
                                               and bool((tok == eos_token_id).all())):
                     logits = self.forward(tok, kv_cache=cache)["logits"][:, -1, :]
                     tok = self._sample(logits, temperature, top_p, top_k, do_sample)
+                    if record is not None:
+                        record.add(logits, tok)
                     out[:, prompt_len + n] = tok[:, 0]
                     n += 1
         finally:
             if own_cache and isinstance(cache, PagedKVCache):
                 cache.free()
-        return out[:, :prompt_len + n]
+        tokens = out[:, :prompt_len + n]
+        return tokens if record is None else (tokens, record.result())
 
     def _decode_graph(self, cache: PagedKVCache, tok, out, prompt_len, max_length, temperature,
-                      top_p, top_k, do_sample) -> int:
+                      top_p, top_k, do_sample, record=None) -> int:
         """Decode steps 2..max_length as replays of one captured HIP graph.  Step 2 runs
         eagerly on the capture stream (warming every kernel and workspace), step 3 is
         captured (capture records without executing), then the graph is replayed."""
@@ -970,22 +1090,27 @@ class Transformer(nn.Module):
         def step():
             logits = self.forward(static_tok, kv_cache=cache)["logits"][:, -1, :]
             static_tok.copy_(self._sample(logits, temperature, top_p, top_k, do_sample))
+            return None if record is None else record.of(logits, static_tok)
 
         n = 1
         try:
             with torch.cuda.stream(stream):
-                step()
+                found = step()
                 cache.advance_host(1)
                 out[:, prompt_len + n] = static_tok[:, 0]
+                if record is not None:
+                    record.keep(found)
                 n += 1
                 if n < max_length:
                     graph = torch.cuda.CUDAGraph()
                     with torch.cuda.graph(graph, stream=stream):
-                        step()  # recorded, not executed: the device state does not move
+                        found = step()  # recorded, not executed: the device state does not move
                     while n < max_length:
                         graph.replay()
                         cache.advance_host(1)
                         out[:, prompt_len + n] = static_tok[:, 0]
+                        if record is not None:
+                            record.keep([t.clone() for t in found])
                         n += 1
             torch.cuda.current_stream(tok.device).wait_stream(stream)
         finally:

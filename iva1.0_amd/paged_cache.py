@@ -255,27 +255,60 @@ class PagedKVPool:
     def fork(self, src_id, dst_id) -> None:
         """New sequence ``dst_id`` with the content of ``src_id``: full pages are shared
         (reference counted), the partial last page is copied into a fresh page."""
+        moved = self._fork_pages(src_id, dst_id)
+        if moved is not None:
+            for t in self.k_pools + self.v_pools + self.k_scales + self.v_scales:
+                t[moved[1]].copy_(t[moved[0]])
+
+    def _fork_pages(self, src_id, dst_id) -> Optional[Tuple[int, int]]:
+        """The bookkeeping of :meth:`fork`; (partial last page, its copy's page) still to copy,
+        or None."""
         s = self._seq(src_id)
         self.add_sequence(dst_id)
         d = self._seqs[dst_id]
         full = s.length // self.block_size
+        moved = None
         try:
             for p in s.pages[:full]:
                 if p >= 0:
                     self._ref[p] += 1
                 d.pages.append(p)
             if s.length % self.block_size:
-                src_page = s.pages[full]
-                new_page = self._take_page()
-                d.pages.append(new_page)
-                for t in self.k_pools + self.v_pools + self.k_scales + self.v_scales:
-                    t[new_page].copy_(t[src_page])
+                moved = (s.pages[full], self._take_page())
+                d.pages.append(moved[1])
         except OutOfPagesError:
             self.free(dst_id)
             raise
         d.length = s.length
         d.reserved = len(d.pages) * self.block_size
         self._sync_row(dst_id)
+        return moved
+
+    def fork_many(self, src_ids: Sequence, dst_ids: Sequence) -> None:
+        """:meth:`fork` of ``src_ids[i]`` into ``dst_ids[i]`` for every i, the partial pages of
+        a layer copied by one launch (ivakv_copy_pages).  Nothing is forked when the pool has too
+        few pages or block-table rows for all."""
+        if len(src_ids) != len(dst_ids):
+            raise ValueError(f"{len(src_ids)} sequences for {len(dst_ids)} forks")
+        need = sum(1 for s in src_ids if self._seq(s).length % self.block_size)
+        if need > len(self._free):
+            raise OutOfPagesError(f"{len(dst_ids)} forks need {need} pages, {len(self._free)} free")
+        if len(dst_ids) > len(self._free_rows):
+            raise OutOfPagesError(f"{len(dst_ids)} forks need as many block-table rows, "
+                                  f"{len(self._free_rows)} of {self.max_seqs} free")
+        taken = [d for d in dst_ids if d in self._seqs]
+        if taken or len(set(dst_ids)) != len(dst_ids):
+            raise ValueError(f"forks into existing or repeated sequences: {taken or list(dst_ids)}")
+        moves = [m for m in map(self._fork_pages, src_ids, dst_ids) if m is not None]
+        if not moves or not self.k_pools:
+            return
+        src, dst = (torch.tensor(x, dtype=torch.int32).to(self.device) for x in zip(*moves))
+        for layer in range(self.num_layers):
+            if self.device.type == "cuda":
+                copy_pages(self.k_pools[layer], self.v_pools[layer], src, dst, **self.scales(layer))
+            else:  # a pool kept on the host
+                for t in (self.k_pools[layer], self.v_pools[layer], *self.scales(layer).values()):
+                    t[dst.long()] = t[src.long()]
 
     def release_outside_window(self, seq_id, window: int, n_sink: int = 0) -> int:
         """Frees the pages of a sequence that hold no position a decode query can still
@@ -396,6 +429,20 @@ class _Slots:
 
 
 @dataclass
+class SharedPrefix:
+    """Groups of a cache's sequences that share their first pages, for
+    ``paged_prefix_decode_attention``."""
+    group_start: torch.Tensor   # int32 [n_groups + 1]
+    prefix_lens: torch.Tensor   # int32 [n_groups], whole pages
+    max_group: int
+    saved_tokens: int           # tokens of K and V per layer that sharing need not read again
+
+    @property
+    def op_args(self) -> tuple:
+        return self.group_start, self.prefix_lens
+
+
+@dataclass
 class LayerView:
     """What one attention layer of one forward gets from a PagedKVCache."""
     layer: int
@@ -407,6 +454,7 @@ class LayerView:
     start: int                   # position of the first new token
     new_tokens: int              # T
     scales: Dict[str, torch.Tensor] = field(default_factory=dict)  # FP8: k_scale / v_scale
+    shared: Optional[SharedPrefix] = None  # groups of sequences forked from one prompt
 
     @property
     def slot_mapping(self) -> torch.Tensor:
@@ -427,7 +475,7 @@ class PagedKVCache:
                  device=None, dtype: torch.dtype = torch.float16, *, num_layers: int = 1,
                  block_size: int = 16, max_seq_len: int = 4096, num_pages: Optional[int] = None,
                  pool: Optional[PagedKVPool] = None, compute_dtype: Optional[torch.dtype] = None,
-                 release_window: bool = True):
+                 release_window: bool = True, max_seqs: Optional[int] = None):
         self.batch_size = int(batch_size)
         # sliding-window attention: pages no later query can see go back to the pool
         # after each forward (release_window), the sink pages stay resident
@@ -446,7 +494,8 @@ class PagedKVCache:
             per_seq = math.ceil(max(int(max_seq_len), int(seq_len), 1) / block_size)
             pages = num_pages if num_pages is not None else per_seq * self.batch_size
             pool = PagedKVPool(pages, self.n_heads, self.head_dim, block_size, self.num_layers,
-                               dtype, self.device, max_seqs=max(self.batch_size, 1),
+                               dtype, self.device,
+                               max_seqs=max(self.batch_size, 1, int(max_seqs or 0)),
                                max_blocks_per_seq=per_seq)
         elif (pool.num_kv_heads, pool.head_dim, pool.num_layers) != (self.n_heads, self.head_dim,
                                                                      self.num_layers):
@@ -462,6 +511,8 @@ class PagedKVCache:
         self._bt_gen = -1      # pool generation the device block table was copied at
         self._static: Optional[dict] = None
         self._positions: Optional[torch.Tensor] = None
+        self.shared: Optional[SharedPrefix] = None   # after fork()
+        self._shared_tokens = 0
         if seq_len > 0:
             z = torch.zeros(self.batch_size, self.n_heads, int(seq_len), self.head_dim,
                             dtype=self.compute_dtype, device=self.device)
@@ -472,10 +523,14 @@ class PagedKVCache:
 
     _next_id = 0
 
+    @staticmethod
+    def _next_number() -> int:
+        PagedKVCache._next_id += 1
+        return PagedKVCache._next_id
+
     def _new_ids(self):
         for _ in range(self.batch_size):
-            PagedKVCache._next_id += 1
-            yield ("cache", PagedKVCache._next_id)
+            yield ("cache", self._next_number())
 
     # ----------------------------------------------------------- duck type
     @property
@@ -540,6 +595,9 @@ class PagedKVCache:
         before any sequence grows."""
         t = new_k.shape[2]
         end = int(start_pos) + t
+        if t and int(start_pos) < self._shared_tokens:
+            raise ValueError(f"positions below {self._shared_tokens} are on pages that forked "
+                             "sequences share")
         layer = self._cursor
         bs = self.pool.block_size
         need = [max(0, -(-end // bs) - len(self.pool.pages(s))) for s in self.seq_ids]
@@ -557,6 +615,37 @@ class PagedKVCache:
                   torch.from_numpy(slots).to(self.device), **self.pool.scales(layer))
         self.seq_len = max(self.seq_len, end)
         self._bt_gen = -1
+
+    def fork(self, samples: int) -> None:
+        """Makes every sequence the first of ``samples`` with the same content, in place: sequence
+        b becomes rows ``b * samples .. (b + 1) * samples - 1`` of the batch.  Full pages are
+        shared, the partial last page is copied (:meth:`PagedKVPool.fork`), and decode steps read
+        the shared pages once per prompt where that pays.  The pool needs block-table rows for
+        the new sequences (``max_seqs``) and a page for each that has a partial one; with fewer,
+        OutOfPagesError is raised with nothing changed."""
+        n = int(samples)
+        if n < 1:
+            raise ValueError(f"samples must be >= 1, got {samples}")
+        if self._view is not None or self._cursor != 0:
+            raise RuntimeError("a forward is in progress on this cache")
+        if self._static is not None:
+            raise RuntimeError("fork() in static decode")
+        if n == 1:
+            return
+        groups = [[s] + [("cache", self._next_number()) for _ in range(n - 1)] for s in self.seq_ids]
+        self.pool.fork_many([g[0] for g in groups for _ in g[1:]], [s for g in groups for s in g[1:]])
+        self.seq_ids = [s for g in groups for s in g]
+        # (a batch forked twice shares what its sequences have in common now)
+        before = self.batch_size
+        self.batch_size *= n
+        self._shared_tokens = self.seq_len // self.block_size * self.block_size
+        self._bt_gen = -1
+        self.shared = None
+        if self._shared_tokens:
+            on = dict(dtype=torch.int32, device=self.device)
+            self.shared = SharedPrefix(torch.arange(0, self.batch_size + 1, n, **on),
+                                       torch.full((before,), self._shared_tokens, **on), n,
+                                       before * (n - 1) * self._shared_tokens)
 
     def free(self) -> None:
         """Returns every page of this cache's sequences to the pool."""
@@ -748,7 +837,7 @@ class PagedKVCache:
         slots, bt, ctx, start, t = self._view
         layer = self._cursor
         return LayerView(layer, self.pool.k_pools[layer], self.pool.v_pools[layer], slots, bt, ctx,
-                         start, t, self.pool.scales(layer))
+                         start, t, self.pool.scales(layer), self.shared)
 
     def _next_layer(self, view: LayerView) -> None:
         self._cursor += 1
