@@ -433,13 +433,13 @@ int ivakv_prefill_attn_split_fp8(const void* q, const void* k_pool, const void* 
  * in ivakv_prefill_attn (rows of a sequence past max_query_len, and rows of no sequence, are
  * left as they are); a row without keys gives zeros.  k_scale / v_scale: the factors of FP8
  * pools (fp16 or bf16 queries), NULL for pools of the queries' type.  Two launches at most, no
- * host synchronisation.  The workspace (ivakv_cross_workspace_size) needs no initialisation;
- * calls that share one must not run concurrently.
+ * host synchronisation.  The workspace (ivakv_cross_workspace_size; fp8: 1 for FP8 pools) needs no
+ * initialisation; calls that share one must not run concurrently.
  * Replaces: AttentionTorch.forward with config.causal False (src/core/attention.py:77-102).
  */
 int ivakv_cross_workspace_size(int batch, int n_tok, int max_query_len, int num_q_heads,
                                int num_kv_heads, int head_dim, int max_blocks, int dtype,
-                               size_t* bytes);
+                               int fp8, size_t* bytes);
 int ivakv_cross_attn(const void* q, const void* k_pool, const void* v_pool, const float* k_scale,
                      const float* v_scale, const int32_t* block_tables, const int32_t* context_lens,
                      const int32_t* query_start, int n_tok, void* out, void* workspace,
@@ -464,7 +464,7 @@ int ivakv_cross_attn(const void* q, const void* k_pool, const void* v_pool, cons
  */
 int ivakv_prefix_workspace_size(int batch, int n_groups, int max_group, int num_q_heads,
                                 int num_kv_heads, int head_dim, int max_blocks, int dtype,
-                                size_t* bytes);
+                                int fp8, size_t* bytes);
 int ivakv_prefix_decode_attn(const void* q, const void* k_pool, const void* v_pool,
                              const float* k_scale, const float* v_scale,
                              const int32_t* block_tables, const int32_t* context_lens,

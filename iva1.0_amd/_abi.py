@@ -183,7 +183,7 @@ SIGNATURES = {
     "ivakv_cross_workspace_size": (c_int, [
         c_int, c_int, c_int, c_int,            # batch, n_tok, max_query_len, num_q_heads
         c_int, c_int, c_int, c_int,            # num_kv_heads, head_dim, max_blocks, dtype
-        POINTER(c_size_t),                     # bytes
+        c_int, POINTER(c_size_t),              # fp8, bytes
     ]),
     "ivakv_cross_attn": (c_int, [
         c_void_p, c_void_p, c_void_p,          # q, k_pool, v_pool
@@ -198,7 +198,7 @@ SIGNATURES = {
     "ivakv_prefix_workspace_size": (c_int, [
         c_int, c_int, c_int, c_int,            # batch, n_groups, max_group, num_q_heads
         c_int, c_int, c_int, c_int,            # num_kv_heads, head_dim, max_blocks, dtype
-        POINTER(c_size_t),                     # bytes
+        c_int, POINTER(c_size_t),              # fp8, bytes
     ]),
     "ivakv_prefix_decode_attn": (c_int, [
         c_void_p, c_void_p, c_void_p,          # q, k_pool, v_pool

@@ -30,7 +30,7 @@
 // fp32 rounded once to the query dtype, into the same LDS layout; the loop over
 // pairs is the 16-bit one.  8-byte units (8 dims of one key of K, or 4 keys of
 // two dims of V) spread the conversion over all threads.
-#include "ivakv_tile.h"
+#include "ivakv_rows.h"
 
 namespace ivakv {
 namespace {
@@ -128,16 +128,16 @@ __device__ inline RowBlock row_block(const PrefillArgs& a, const int32_t* ctx, c
   return rb;
 }
 
-// Row block xb of (sequence b, kv head h) over pairs [pair_lo, pair_hi) of its walk
-// (pair_lo even).  slot < 0: the block's whole walk, normalized rows into out; slot
+// Row block blk of (sequence b, kv head h) over pairs [pair_lo, pair_hi) of its walk
+// (pair_lo even).  kCausal false: every row sees all blk.L keys.  slot < 0: the block's whole walk, normalized rows into out; slot
 // >= 0: one segment of a split walk, its unnormalized rows (acc, running max, row sum)
 // into partial slot `slot` of the split workspace, for merge_rows.  Every
 // thread of the workgroup calls it with the same arguments (the returns and barriers
 // inside are uniform).
-template <int DT, int D, bool kFp8, bool kSplit>
+template <int DT, int D, bool kFp8, bool kSplit, bool kCausal = true>
 __device__ __attribute__((always_inline)) inline void prefill_rows(
-    const PrefillArgs& a, const int32_t* __restrict__ bt, const int32_t* __restrict__ ctx,
-    const int32_t* __restrict__ qstart, int b, int h, int xb, int pair_lo, int pair_hi, int slot) {
+    const PrefillArgs& a, const int32_t* __restrict__ bt, const RowBlock& blk, int b, int h,
+    int pair_lo, int pair_hi, int slot) {
   using Tr = Traits<DT>;
   using E = typename Tr::E;
   using S = PrefillShape<DT, D, kSplit>;
@@ -154,7 +154,6 @@ __device__ __attribute__((always_inline)) inline void prefill_rows(
   const int lane = tid & 63, ln = lane & 15, lq = lane >> 4;
   const int wave = uni(tid >> 6);
   const int G = a.G, Hkv = a.Hkv, Hq = Hkv * G;
-  const RowBlock blk = row_block(a, ctx, qstart, b, xb, S::kRowsWG);
   if (!blk.ok) return;  // uniform over the workgroup
   const int q0 = blk.q0, L = blk.L, rows = blk.rows, r_wg = blk.r_wg, first_pos = blk.first_pos;
   const PageWalk w = blk.w;
@@ -169,13 +168,14 @@ __device__ __attribute__((always_inline)) inline void prefill_rows(
   // This wave's rows: the last position any of them has (pairs entirely past it
   // are skipped) and, per lane, the position of row ln of each block.
   const int r_w = r_wg + wave * S::kRowsWave;
-  const int wave_p_hi = r_w < rows ? first_pos + (min(r_w + S::kRowsWave, rows) - 1) / G : -1;
+  const int wave_p_hi =
+      r_w >= rows ? -1 : kCausal ? first_pos + (min(r_w + S::kRowsWave, rows) - 1) / G : L - 1;
   int qpos[NR];
   Chunk16 qr[NR][KLD];
 #pragma unroll
   for (int rb = 0; rb < NR; ++rb) {
     const int r = r_w + 16 * rb + ln;
-    const int pos = first_pos + r / G;
+    const int pos = kCausal ? first_pos + r / G : L - 1;
     qpos[rb] = (r < rows && pos >= 0) ? pos : -1;
     const int rc = r < rows ? r : 0;
     const E* qb = static_cast<const E*>(a.q) + ((int64_t)(q0 + rc / G) * Hq + h * G + rc % G) * D;
@@ -541,7 +541,7 @@ __device__ __attribute__((always_inline)) inline void prefill_rows(
   // the chunk's end read row 0's query, so their scores stay finite; they are
   // never stored.)  Past the sink pages logical pages are consecutive, so these are the
   // pairs [int_lo, int_hi); pairs with sink pages before a window are masked.
-  const int wave_pos_lo = first_pos + r_w / G;  // may be negative: then no pair is
+  const int wave_pos_lo = kCausal ? first_pos + r_w / G : L - 1;  // may be negative: then no pair is
   const int d_lp = w.win_first - w.sink_pages;
   int int_lo = (w.sink_pages + 1) >> 1, int_hi = 0;
   if (a.window > 0 && wave_p_hi - a.window >= 0)
@@ -709,7 +709,8 @@ void prefill_kernel(PrefillArgs a,
   if (unit >= a.batch * a.Hkv) return;
   const int b = unit / a.Hkv, h = unit % a.Hkv;
   const int xb = a.blocks_x - 1 - slot % a.blocks_x;
-  prefill_rows<DT, D, kFp8, false>(a, bt, ctx, qstart, b, h, xb, 0, 0x7fffffff, -1);
+  const RowBlock blk = row_block(a, ctx, qstart, b, xb, PrefillShape<DT, D, false>::kRowsWG);
+  prefill_rows<DT, D, kFp8, false>(a, bt, blk, b, h, 0, 0x7fffffff, -1);
 }
 
 // ---------------------------------------------------------------------------
@@ -1027,12 +1028,12 @@ __global__ __launch_bounds__((PrefillShape<DT, D, true>::kThreads)) void prefill
     const int b = vu.x & 0xffff, h = vu.x >> 16, s = vu.y;
     const int2 rb = ws.rb[b * a.blocks_x + xb];
     if (s >= rb.y) continue;  // the block has no rows, or fewer segments
+    const RowBlock rows = row_block(a, ctx, qstart, b, xb, S::kRowsWG);
     if (rb.y == 1) {
-      prefill_rows<DT, D, kFp8, true>(a, bt, ctx, qstart, b, h, xb, 0, 0x7fffffff, -1);
+      prefill_rows<DT, D, kFp8, true>(a, bt, rows, b, h, 0, 0x7fffffff, -1);
       continue;
     }
-    prefill_rows<DT, D, kFp8, true>(a, bt, ctx, qstart, b, h, xb, s * seg, (s + 1) * seg,
-                                    rb.x + h * rb.y + s);
+    prefill_rows<DT, D, kFp8, true>(a, bt, rows, b, h, s * seg, (s + 1) * seg, rb.x + h * rb.y + s);
     // Count the segment in: every wave waits until its partial stores have reached this
     // XCD's L2 (the barrier alone waits only for LDS traffic), then thread 0's
     // agent-scope release writes them back where the other XCDs read, and the arrival
@@ -1059,6 +1060,67 @@ __global__ __launch_bounds__((PrefillShape<DT, D, true>::kThreads)) void prefill
       merge_rows<DT, D>(a, ws, blk, h2, first, rb2.y, S::kRowsWG);
     }
   }
+}
+
+// The shared walk of ivakv_rows.hip for many rows: a workgroup takes up to kRowsWG rows of a group and
+// a piece of its pages, staged through LDS once for all of them, and leaves one partial (or, where
+// cross attention does not cut, the finished rows).
+template <int DT, int D>
+__global__ __launch_bounds__((PrefillShape<DT, D, true>::kThreads)) void rows_wide_kernel(
+    RowArgs a, const int32_t* __restrict__ bt) {
+  using S = PrefillShape<DT, D, true>;
+  const int lane = threadIdx.x & 63;
+  const Group own = load_group(a, lane);
+  const Pieces pc(a, own, lane);
+  const int n_wg = pc.items * a.Hkv;
+  if ((int)blockIdx.x >= n_wg) return;
+  const int wg = (int)xcd_contiguous_block(blockIdx.x, n_wg);
+  Group group;
+  int g, piece, h, chunk;
+  if (!pc.find(a, own, wg, lane, group, g, piece, h, chunk)) return;
+  const int table = a.prefix ? prefix_row(a, group.pages, group.r0, group.r1, lane) : g;
+  if (table < 0) return;
+  RowBlock blk;
+  blk.ok = true;
+  blk.q0 = group.r0;
+  blk.rows = min(group.r1 - group.r0, a.max_rows) * a.G;
+  blk.L = a.prefix ? group.pages * kBS : max(a.ctx[g], 0);
+  blk.first_pos = 0;
+  blk.r_wg = chunk * S::kRowsWG;
+  blk.w = make_walk(blk.L, 0, 0, kBS);
+  blk.n_eff = table_pages(blk.w, a.max_blocks, kBS);
+  blk.n_pairs = (blk.n_eff + 1) / 2;
+  PrefillArgs p{};
+  p.q = a.q;
+  p.k_pool = a.k_pool;
+  p.v_pool = a.v_pool;
+  p.out = a.out;
+  p.n_tok = a.n_rows;
+  p.Hkv = a.Hkv;
+  p.G = a.G;
+  p.max_blocks = a.max_blocks;
+  p.num_pages = a.num_pages;
+  p.scale_log2 = a.scale_log2;
+  p.part_acc = a.part_acc;
+  p.part_ml = a.part_ml;
+  const bool whole = !a.prefix && pc.of(group) == 1;
+  const int lo = piece * (pc.len / 2);
+  prefill_rows<DT, D, false, true, false>(p, bt, blk, table, h, lo, min(lo + pc.len / 2, blk.n_pairs),
+                                          whole ? -1 : wg);
+}
+
+template <int DT, int D>
+void launch_wide_d(const RowArgs& a, hipStream_t stream) {
+  using S = PrefillShape<DT, D, true>;
+  static std::atomic<uint64_t> done{0};
+  allow_lds(reinterpret_cast<const void*>(&rows_wide_kernel<DT, D>), (int)S::kLdsBytes, done);
+  rows_wide_kernel<DT, D><<<a.shared_wgs, S::kThreads, S::kLdsBytes, stream>>>(a, a.bt);
+}
+
+template <int DT>
+void launch_wide(int head_dim, const RowArgs& a, hipStream_t stream) {
+  if (head_dim == 128) launch_wide_d<DT, 128>(a, stream);
+  else launch_wide_d<DT, 256>(a, stream);
 }
 
 template <int DT, int D, bool kFp8>
@@ -1239,6 +1301,14 @@ int prefill_entry(const char* name, const void* q, const void* k_pool, const voi
 }
 
 }  // namespace
+
+int wide_rows(int head_dim) { return rows_per_workgroup(IVAKV_F16, head_dim); }
+
+void launch_rows_wide(int dtype, int head_dim, const RowArgs& a, hipStream_t stream) {
+  if (dtype == IVAKV_F16) launch_wide<IVAKV_F16>(head_dim, a, stream);
+  else launch_wide<IVAKV_BF16>(head_dim, a, stream);
+}
+
 }  // namespace ivakv
 
 using namespace ivakv;

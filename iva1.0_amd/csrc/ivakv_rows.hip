@@ -26,40 +26,13 @@
 // pages; from a few hundred rows on the matrix and vector pipes (4 D operations per key and row).
 #include <type_traits>
 
-#include "ivakv_tile.h"
+#include "ivakv_rows.h"
 
 namespace ivakv {
 namespace {
 
 // Log2-domain headroom of the lazy row max, as in the prefill: p = exp2(s - m) stays <= 2^8.
 constexpr float kLazyMax = 8.f;
-
-struct RowArgs {
-  const void* q;  // [n_rows, Hq, D]
-  const void* k_pool;
-  const void* v_pool;
-  const float* k_scale;  // FP8 pools
-  const float* v_scale;
-  void* out;             // like q
-  const int32_t* bt;     // [tables, max_blocks]
-  const int32_t* ctx;    // cross: keys of each group; prefix: length of each row's sequence
-  const int32_t* start;  // [n_groups + 1] first query row of each group
-  const int32_t* shared; // prefix: [n_groups] shared tokens
-  float* part_acc;       // shared partials [slot][16 NR][D]
-  float* part_ml;        // [slot][16 NR][2]  (running max, sum)
-  float* own_acc;        // own partials [slot][G][D]
-  float* own_ml;         // [slot][G][2]
-  int32_t* own_pref;     // [n_rows + 1] own page sets before each row
-  int n_groups, n_rows, Hkv, G, max_blocks, num_pages;
-  int prefix;            // 1: prefix groups, 0: cross
-  int max_rows;          // query rows of the largest group
-  int rows_shift;        // log2 of the rows of a chunk (16 NR)
-  int items, split;      // (piece, row chunk) pairs the grid holds for a kv head; whether pages are cut
-  int unit;              // pages a shared workgroup's waves take at once
-  int shared_wgs, own_waves;  // workgroups of the shared walk, waves of the own walk
-  float scale_log2;
-  int window, n_sink;
-};
 
 // Register tile of one page (lane = 16 lq + ln) and its products, for pools of the queries' type.
 template <int DT, int D, bool kFp8>
@@ -556,140 +529,6 @@ __device__ inline void join_waves(const WalkT& wk, float* smem, int wave, int ln
   __syncthreads();
 }
 
-// Rows [r0, r1) of group g, inside [0, n_rows].
-__device__ inline void group_rows(const RowArgs& a, int g, int& r0, int& r1) {
-  r0 = min(max(a.start[g], 0), a.n_rows);
-  r1 = min(max(a.start[g + 1], r0), a.n_rows);
-}
-
-// One group as a lane holds it: its rows, their chunks and its pages.  prefix: the full pages of the
-// shared tokens, inside the table.  A group without rows has no chunks.
-struct Group {
-  int r0, r1, chunks, pages;
-};
-__device__ inline Group load_group(const RowArgs& a, int g) {
-  Group x{0, 0, 0, 0};
-  if (g >= a.n_groups) return x;
-  const int n = a.prefix ? a.shared[g] / kBS : cdiv(max(a.ctx[g], 0), kBS);
-  group_rows(a, g, x.r0, x.r1);
-  x.chunks = (min(x.r1 - x.r0, a.max_rows) * a.G + (1 << a.rows_shift) - 1) >> a.rows_shift;
-  x.pages = x.chunks > 0 ? min(max(n, 0), a.max_blocks) : 0;
-  return x;
-}
-
-// Whether a sequence of length len takes part in its group's shared walk of `blocks` pages: it has
-// the whole prefix and its window cuts nothing off.  (Any other row walks all of its visible pages
-// itself, so the shared walk needs no mask of its own.)
-__device__ inline bool takes_part(const RowArgs& a, int len, int blocks) {
-  return len >= blocks * kBS && (a.window <= 0 || len <= a.window);
-}
-
-// The first row of [r0, r1) that takes part, whose table the shared walk reads (-1: none, and then no
-// row asks for the walk's partials).
-__device__ inline int prefix_row(const RowArgs& a, int blocks, int r0, int r1, int lane) {
-  for (int r = r0; r < r1; r += 64) {
-    const uint64_t has =
-        __builtin_amdgcn_ballot_w64(r + lane < r1 && takes_part(a, a.ctx[min(r + lane, r1 - 1)], blocks));
-    if (has != 0) return r + __builtin_ctzll(has);
-  }
-  return -1;
-}
-
-// Inclusive scan over the wave's lanes (row shifts, then the rows' last lanes broadcast).
-__device__ inline int wave_scan(int x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);
-  return x;
-}
-__device__ inline int wave_sum(int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
-
-// How the groups' pages are cut: every list into pieces of `len` pages (a multiple of the pages that a
-// workgroup's waves take at once), the shortest of four lengths with which all groups' items, pieces
-// times row chunks, number at most a.items.  The last of the four, sum (pages x chunks) / (items -
-// sum chunks), always does: a group has at most one piece that is not whole.  Without a.split
-// every group is one piece.  Partials, and the shared workgroups, are numbered group by group, in it
-// piece by piece, kv head by kv head, chunk by chunk.  A cross group without keys has one empty
-// piece, which writes its rows' zeros.  Each wave works this out for itself, 64 groups at a time,
-// the first 64 (`own`, group `lane`) from registers.
-struct Pieces {
-  int len, least, items;  // items: of all groups
-  __device__ inline int of(const Group& x) const {
-    return x.chunks == 0 ? 0 : max((int)(((uint32_t)x.pages + (uint32_t)len - 1) / (uint32_t)len), least);
-  }
-
-  __device__ inline Pieces(const RowArgs& a, const Group& own, int lane) {
-    least = a.prefix ? 0 : 1;
-    len = 1 << 30;
-    int work = 0, chunks = 0;
-    if (a.split) {  // (then items x max_blocks, and so the work, is below 2^31)
-      work = wave_sum(own.pages * own.chunks);
-      chunks = wave_sum(own.chunks);
-      for (int g0 = 64; g0 < a.n_groups; g0 += 64) {
-        const Group x = load_group(a, g0 + lane);
-        work += wave_sum(x.pages * x.chunks);
-        chunks += wave_sum(x.chunks);
-      }
-    }
-#pragma unroll 1
-    for (int k = a.split ? 0 : 3; k < 4; ++k) {
-      if (a.split) {
-        const uint32_t parts = (uint32_t)max(a.items - k * chunks / 3, 1), unit = (uint32_t)a.unit;
-        len = (int)max(((uint32_t)work + parts * unit - 1) / (parts * unit) * unit, unit);
-      }
-      items = wave_sum(of(own) * own.chunks);
-      for (int g0 = 64; g0 < a.n_groups; g0 += 64) {
-        const Group x = load_group(a, g0 + lane);
-        items += wave_sum(of(x) * x.chunks);
-      }
-      if (items <= a.items) return;
-    }
-  }
-
-  // What shared workgroup `wg` does: the group, which of its pieces, kv head and chunk; false when
-  // there is nothing for it.
-  __device__ inline bool find(const RowArgs& a, const Group& own, int wg, int lane, Group& group, int& g, int& piece,
-                              int& h, int& chunk) const {
-    int before = 0;
-    for (int g0 = 0; g0 < a.n_groups; g0 += 64) {
-      const Group x = g0 == 0 ? own : load_group(a, g0 + lane);
-      const int n = of(x) * x.chunks * a.Hkv, incl = wave_scan(n);
-      const uint64_t has = __builtin_amdgcn_ballot_w64(wg < before + incl);
-      if (has != 0) {
-        const int w = __builtin_ctzll(has);
-        g = g0 + w;
-        group = Group{__builtin_amdgcn_readlane(x.r0, w), __builtin_amdgcn_readlane(x.r1, w),
-                      __builtin_amdgcn_readlane(x.chunks, w), __builtin_amdgcn_readlane(x.pages, w)};
-        const uint32_t at = (uint32_t)(wg - before - (__builtin_amdgcn_readlane(incl, w) - __builtin_amdgcn_readlane(n, w)));
-        chunk = (int)(at % (uint32_t)group.chunks);
-        const uint32_t ph = at / (uint32_t)group.chunks;
-        h = (int)(ph % (uint32_t)a.Hkv);
-        piece = (int)(ph / (uint32_t)a.Hkv);
-        return true;
-      }
-      before += __builtin_amdgcn_readlane(incl, 63);
-    }
-    return false;
-  }
-
-  // First partial of group g, and its pieces.
-  __device__ inline void of_group(const RowArgs& a, const Group& own, int g, int lane, int64_t& first,
-                                  int& pieces) const {
-    int before = 0, n = 0, mine = 0;
-    for (int g0 = 0; g0 <= g; g0 += 64) {
-      const Group x = g0 == 0 ? own : load_group(a, g0 + lane);
-      mine = of(x);
-      n = g0 + lane <= g ? mine * x.chunks : 0;
-      before += wave_sum(n);
-    }
-    pieces = __builtin_amdgcn_readlane(mine, g & 63);
-    first = (int64_t)(before - __builtin_amdgcn_readlane(n, g & 63)) * a.Hkv;
-  }
-};
-
 // Workgroups of the walks: four waves of 256 registers, two workgroups per CU (a shared one and one
 // of the own walk, say); rows of 512 bytes need 512 registers.
 template <int DT, int D, bool kFp8, int NR>
@@ -1069,27 +908,43 @@ int num_cus() {
   return cus;
 }
 
-constexpr int kSharedPerCU = 1;
-
 struct Plan {
-  int nr, chunks, items, own_waves;
-  bool split;
+  int nr, rows_chunk, chunks, items, own_waves;
+  bool split, wide;
 };
 
-// Row chunks and items of a launch: kSharedPerCU shared workgroups per CU, at least one per group and
-// chunk (then nothing is cut).  The own
-// walk (own_sets > 0: the sets of pages it has at most) gets a wave per SIMD, the other half of the CU
-// (two: 64 rows on FP8 pages 55.6 against 51.6 us, 256 rows 154 against 142).
-Plan make_plan(int row_bytes, int n_groups, int64_t max_rows, int hkv, int g, int64_t own_sets,
-               int max_blocks) {
+// Whether a group's shared walk goes through LDS in chunks of up to 256 rows (wide) rather than through
+// the waves' own registers in chunks of 32.  It reads the pages from the L2 once for eight times the
+// rows, but leaves a partial of all rows per piece and has one workgroup per CU to hide a piece's
+// start and end.  So it takes cross attention where whole chunks need no cutting into pieces (fp16,
+// D 128, walk : wide in us: 8 sequences of 200 x 2000, 32 / 8 heads 105 : 79, 16 of 97 .. 448 x 700 ..
+// 1500 200 : 151; cut in two, 16 of 64 x 1000 .. 1500 57 : 73), and a prefix long for its rows (768 rows on
+// 8192 tokens 81 : 69, 1024 on 16384 155 : 128; 512 on 8192 49 : 57, 1024 on 2048 47 : 58).  At head_dim
+// 64 the softmax bounds both (16 of 448 x 1500, 16 heads 79 : 87).  FP8 pages would be rounded to the
+// queries' type on the way.
+bool wide_walk(int head_dim, int dtype, bool fp8, bool prefix, int n_groups, int64_t rows, int hkv, int max_blocks) {
+  if (fp8 || dtype == IVAKV_F32 || head_dim < 128 || rows < 256) return false;
+  const int64_t chunk = wide_rows(head_dim);
+  return prefix ? rows * max_blocks >= 5 << 16 : n_groups * ((rows + chunk - 1) / chunk) * hkv >= num_cus();
+}
+
+// Row chunks and items of a launch: a shared workgroup per CU, at least one per group and chunk (then
+// nothing is cut).  The own walk (own_sets > 0: the sets of pages it has at most) gets a wave per
+// SIMD, the other half of the CU (two: 64 rows on FP8 pages 55.6 against 51.6 us, 256 rows 154
+// against 142), or two in a launch of its own.
+Plan make_plan(int head_dim, int dtype, bool fp8, bool prefix, int n_groups, int64_t max_rows, int hkv, int g,
+               int64_t own_sets, int max_blocks) {
   Plan p;
   const int64_t rows = n_groups > 0 ? max_rows * g : 0;
-  p.nr = row_blocks(row_bytes, rows);
-  p.chunks = (int)((rows + 16 * p.nr - 1) / (16 * p.nr));
-  const int64_t least = (int64_t)n_groups * p.chunks, most = num_cus() * kSharedPerCU / hkv;
+  const int row_bytes = head_dim * dtype_size(dtype);
+  p.wide = wide_walk(head_dim, dtype, fp8, prefix, n_groups, rows, hkv, max_blocks);
+  p.nr = row_blocks(row_bytes, p.wide ? 1 : rows);
+  p.rows_chunk = p.wide ? wide_rows(head_dim) : 16 * p.nr;
+  p.chunks = (int)((rows + p.rows_chunk - 1) / p.rows_chunk);
+  const int64_t least = (int64_t)n_groups * p.chunks, most = num_cus() / hkv;
   p.split = p.chunks > 0 && most > least && most * max_blocks < 0x7fffffff;
   p.items = p.split ? (int)most : least < 0x7fffffff ? (int)least : 0x7fffffff;
-  const int64_t waves = (int64_t)num_cus() * 4, want = ((own_sets + 1) / 2 + 3) & ~3ll;
+  const int64_t waves = (int64_t)num_cus() * (p.wide ? 8 : 4), want = ((own_sets + 1) / 2 + 3) & ~3ll;
   p.own_waves = (int)(want < waves ? want : waves);
   return p;
 }
@@ -1100,7 +955,7 @@ struct Layout {
 };
 Layout make_layout(const Plan& p, int n_rows, int hkv, int g, int d) {
   Layout l;
-  const size_t rows = p.split || p.own_waves > 0 ? (size_t)p.items * hkv * 16 * p.nr : 0;
+  const size_t rows = p.split || p.own_waves > 0 ? (size_t)p.items * hkv * p.rows_chunk : 0;
   const size_t own = p.own_waves > 0 ? ((size_t)p.own_waves + (size_t)n_rows * hkv) * g : 0;
   l.part_ml = rows * d;
   l.own_acc = l.part_ml + rows * 2;
@@ -1121,14 +976,21 @@ void launch_walk_n(RowArgs a, hipStream_t stream) {
 }
 
 template <int DT, int D, bool kFp8>
-void launch_d(int nr, bool shared_chunks, RowArgs a, hipStream_t stream) {
+void launch_d(const Plan& p, RowArgs a, hipStream_t stream) {
+  const int nr = p.nr;
+  const bool shared_chunks = p.chunks > 1;
   constexpr int most = max_row_blocks(Shape<DT, D, kFp8, 1>::kRow);
   a.unit = 4 * PageOps<DT, D, kFp8>::kPages;
   a.shared_wgs = a.items * a.Hkv;
+  if (p.wide) {  // the shared walk in a launch of its own
+    a.unit = 4;  // (two page pairs: the staged walk starts at even ones)
+    launch_rows_wide(DT, D, a, stream);
+    a.shared_wgs = 0;
+  }
   // One chunk reads every page once: streaming loads.  Several share them through the L2.
   if (a.shared_wgs + a.own_waves == 0) {
-    // nothing to walk: the join writes zeros
-  } else if (nr == most && shared_chunks) {
+    // nothing (more) to walk
+  } else if (nr == most && shared_chunks && !p.wide) {
     launch_walk_n<DT, D, kFp8, most, false>(a, stream);
   } else if (nr == 1) {
     launch_walk_n<DT, D, kFp8, 1, true>(a, stream);
@@ -1141,24 +1003,24 @@ void launch_d(int nr, bool shared_chunks, RowArgs a, hipStream_t stream) {
 }
 
 template <int DT, bool kFp8>
-void launch_t(int head_dim, int nr, bool shared_chunks, const RowArgs& a, hipStream_t stream) {
+void launch_t(int head_dim, const Plan& p, const RowArgs& a, hipStream_t stream) {
   switch (head_dim) {
-    case 64: launch_d<DT, 64, kFp8>(nr, shared_chunks, a, stream); break;
-    case 128: launch_d<DT, 128, kFp8>(nr, shared_chunks, a, stream); break;
-    default: launch_d<DT, 256, kFp8>(nr, shared_chunks, a, stream); break;
+    case 64: launch_d<DT, 64, kFp8>(p, a, stream); break;
+    case 128: launch_d<DT, 128, kFp8>(p, a, stream); break;
+    default: launch_d<DT, 256, kFp8>(p, a, stream); break;
   }
 }
 
-void launch(int dtype, bool fp8, int head_dim, int nr, bool shared_chunks, const RowArgs& a, hipStream_t stream) {
+void launch(int dtype, bool fp8, int head_dim, const Plan& p, const RowArgs& a, hipStream_t stream) {
   if (fp8) {
-    if (dtype == IVAKV_F16) launch_t<IVAKV_F16, true>(head_dim, nr, shared_chunks, a, stream);
-    else launch_t<IVAKV_BF16, true>(head_dim, nr, shared_chunks, a, stream);
+    if (dtype == IVAKV_F16) launch_t<IVAKV_F16, true>(head_dim, p, a, stream);
+    else launch_t<IVAKV_BF16, true>(head_dim, p, a, stream);
     return;
   }
   switch (dtype) {
-    case IVAKV_F16: launch_t<IVAKV_F16, false>(head_dim, nr, shared_chunks, a, stream); break;
-    case IVAKV_BF16: launch_t<IVAKV_BF16, false>(head_dim, nr, shared_chunks, a, stream); break;
-    default: launch_t<IVAKV_F32, false>(head_dim, nr, shared_chunks, a, stream); break;
+    case IVAKV_F16: launch_t<IVAKV_F16, false>(head_dim, p, a, stream); break;
+    case IVAKV_BF16: launch_t<IVAKV_BF16, false>(head_dim, p, a, stream); break;
+    default: launch_t<IVAKV_F32, false>(head_dim, p, a, stream); break;
   }
 }
 
@@ -1178,9 +1040,8 @@ int check_geometry(const char* name, int n_groups, int num_q_heads, int num_kv_h
 }
 
 Plan plan_of(int n_groups, int n_rows, int num_q_heads, int num_kv_heads, int head_dim, int max_rows, int dtype,
-             int max_blocks, bool prefix) {
-  const int row_bytes = head_dim * dtype_size(dtype);
-  return make_plan(row_bytes, n_groups, max_rows, num_kv_heads, num_q_heads / num_kv_heads,
+             bool fp8, int max_blocks, bool prefix) {
+  return make_plan(head_dim, dtype, fp8, prefix, n_groups, max_rows, num_kv_heads, num_q_heads / num_kv_heads,
                    prefix ? (int64_t)n_rows * num_kv_heads * max_blocks : 0, max_blocks);
 }
 
@@ -1218,8 +1079,8 @@ int rows_entry(const char* name, RowArgs a, int batch, int num_q_heads, int head
     return fail(IVAKV_E_SHAPE, "%s: at most %d rows, and rows x max_blocks x num_kv_heads below 2^31 (got %d, %d, %d)",
                 name, kMaxBatch, a.n_rows, a.max_blocks, a.Hkv);
   a.max_rows = a.max_rows < a.n_rows ? a.max_rows : a.n_rows;
-  const Plan p = plan_of(a.n_groups, a.n_rows, num_q_heads, a.Hkv, head_dim, a.max_rows, dtype, a.max_blocks,
-                         a.prefix);
+  const Plan p = plan_of(a.n_groups, a.n_rows, num_q_heads, a.Hkv, head_dim, a.max_rows, dtype, fp8,
+                         a.max_blocks, a.prefix);
   const int bad = check_plan(name, p, a.Hkv);
   if (bad != IVAKV_OK) return bad;
   const Layout l = make_layout(p, a.n_rows, a.Hkv, a.G, head_dim);
@@ -1227,7 +1088,8 @@ int rows_entry(const char* name, RowArgs a, int batch, int num_q_heads, int head
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
     return fail(IVAKV_E_WORKSPACE, "%s: workspace of %zu bytes (16-byte aligned) required, got %zu", name, need,
                 workspace ? workspace_bytes : (size_t)0);
-  a.rows_shift = p.nr == 1 ? 4 : p.nr == 2 ? 5 : 6;
+  a.rows_shift = 0;
+  while ((1 << a.rows_shift) < p.rows_chunk) ++a.rows_shift;
   a.items = p.items;
   a.split = p.split;
   a.own_waves = p.own_waves;
@@ -1238,12 +1100,12 @@ int rows_entry(const char* name, RowArgs a, int batch, int num_q_heads, int head
   a.own_pref = reinterpret_cast<int32_t*>(a.part_acc + l.own_pref);
   a.scale_log2 = (float)((double)scale * 1.4426950408889634);
   a.window = a.window > 0 ? a.window : 0;
-  launch(dtype, fp8, head_dim, p.nr, p.chunks > 1, a, stream);
+  launch(dtype, fp8, head_dim, p, a, stream);
   return launch_status(name);
 }
 
 int workspace_size(const char* name, int n_groups, int n_rows, int num_q_heads, int num_kv_heads, int head_dim,
-                   int max_rows, int dtype, int max_blocks, bool prefix, size_t* bytes) {
+                   int max_rows, int dtype, bool fp8, int max_blocks, bool prefix, size_t* bytes) {
   if (!bytes) return fail(IVAKV_E_ARG, "%s: null bytes", name);
   *bytes = 0;
   const int err = check_geometry(name, n_groups, num_q_heads, num_kv_heads, head_dim, max_rows, dtype);
@@ -1251,7 +1113,7 @@ int workspace_size(const char* name, int n_groups, int n_rows, int num_q_heads, 
   if (n_rows < 0 || max_blocks < 0)
     return fail(IVAKV_E_ARG, "%s: bad sizes rows=%d max_blocks=%d", name, n_rows, max_blocks);
   const Plan p = plan_of(n_groups, n_rows, num_q_heads, num_kv_heads, head_dim,
-                         max_rows < n_rows ? max_rows : n_rows, dtype, max_blocks, prefix);
+                         max_rows < n_rows ? max_rows : n_rows, dtype, fp8, max_blocks, prefix);
   const int bad = check_plan(name, p, num_kv_heads);
   if (bad != IVAKV_OK) return bad;
   *bytes = make_layout(p, n_rows, num_kv_heads, num_q_heads / num_kv_heads, head_dim).total * sizeof(float);
@@ -1264,10 +1126,10 @@ int workspace_size(const char* name, int n_groups, int n_rows, int num_q_heads, 
 using namespace ivakv;
 
 extern "C" int ivakv_prefix_workspace_size(int batch, int n_groups, int max_group, int num_q_heads,
-                                           int num_kv_heads, int head_dim, int max_blocks, int dtype,
+                                           int num_kv_heads, int head_dim, int max_blocks, int dtype, int fp8,
                                            size_t* bytes) {
   return workspace_size("ivakv_prefix_workspace_size", n_groups, batch, num_q_heads, num_kv_heads, head_dim,
-                        max_group, dtype, max_blocks, true, bytes);
+                        max_group, dtype, fp8 != 0, max_blocks, true, bytes);
 }
 
 extern "C" int ivakv_prefix_decode_attn(const void* q, const void* k_pool, const void* v_pool,
@@ -1303,10 +1165,10 @@ extern "C" int ivakv_prefix_decode_attn(const void* q, const void* k_pool, const
 }
 
 extern "C" int ivakv_cross_workspace_size(int batch, int n_tok, int max_query_len, int num_q_heads,
-                                          int num_kv_heads, int head_dim, int max_blocks, int dtype,
+                                          int num_kv_heads, int head_dim, int max_blocks, int dtype, int fp8,
                                           size_t* bytes) {
   return workspace_size("ivakv_cross_workspace_size", batch, n_tok, num_q_heads, num_kv_heads, head_dim,
-                        max_query_len, dtype, max_blocks, false, bytes);
+                        max_query_len, dtype, fp8 != 0, max_blocks, false, bytes);
 }
 
 extern "C" int ivakv_cross_attn(const void* q, const void* k_pool, const void* v_pool, const float* k_scale,

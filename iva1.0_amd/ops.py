@@ -767,12 +767,12 @@ def _row_workspace_bytes(entry: str, *geometry: int) -> int:
 
 def cross_workspace_bytes(batch: int, n_tok: int, max_query_len: int, num_q_heads: int,
                           num_kv_heads: int, head_dim: int, max_blocks: int,
-                          dtype: torch.dtype) -> int:
-    """Workspace bytes of :func:`paged_cross_attention` (``dtype`` of the queries).  The workspace
-    needs no initialisation."""
+                          dtype: torch.dtype, fp8: bool = False) -> int:
+    """Workspace bytes of :func:`paged_cross_attention` (``dtype`` of the queries, ``fp8``: FP8
+    pools).  The workspace needs no initialisation."""
     return _row_workspace_bytes("ivakv_cross_workspace_size", int(batch), int(n_tok),
                                 int(max_query_len), int(num_q_heads), int(num_kv_heads),
-                                int(head_dim), int(max_blocks), dtype_code(dtype))
+                                int(head_dim), int(max_blocks), dtype_code(dtype), int(fp8))
 
 
 def paged_cross_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
@@ -807,7 +807,8 @@ def paged_cross_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.T
     if scale is None:
         scale = 1.0 / math.sqrt(head_dim)
     workspace = _sized_workspace(workspace, dev, cross_workspace_bytes(
-        batch, n_tok, max_query_len, hq, hkv, head_dim, block_tables.shape[1], q.dtype))
+        batch, n_tok, max_query_len, hq, hkv, head_dim, block_tables.shape[1], q.dtype,
+        scales[0] is not None))
     _abi.call("ivakv_cross_attn", q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), *scales,
               block_tables.data_ptr(), context_lens.data_ptr(), query_start.data_ptr(), n_tok,
               out.data_ptr(), workspace.data_ptr(), workspace.numel() * workspace.element_size(),
@@ -818,12 +819,12 @@ def paged_cross_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.T
 
 def prefix_workspace_bytes(batch: int, n_groups: int, max_group: int, num_q_heads: int,
                            num_kv_heads: int, head_dim: int, max_blocks: int,
-                           dtype: torch.dtype) -> int:
-    """Workspace bytes of :func:`paged_prefix_decode_attention` (``dtype`` of the queries).  The
-    workspace needs no initialisation."""
+                           dtype: torch.dtype, fp8: bool = False) -> int:
+    """Workspace bytes of :func:`paged_prefix_decode_attention` (``dtype`` of the queries,
+    ``fp8``: FP8 pools).  The workspace needs no initialisation."""
     return _row_workspace_bytes("ivakv_prefix_workspace_size", int(batch), int(n_groups),
                                 int(max_group), int(num_q_heads), int(num_kv_heads),
-                                int(head_dim), int(max_blocks), dtype_code(dtype))
+                                int(head_dim), int(max_blocks), dtype_code(dtype), int(fp8))
 
 
 def paged_prefix_decode_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
@@ -866,7 +867,8 @@ def paged_prefix_decode_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool:
     if scale is None:
         scale = 1.0 / math.sqrt(head_dim)
     workspace = _sized_workspace(workspace, dev, prefix_workspace_bytes(
-        batch, n_groups, max_group, hq, hkv, head_dim, block_tables.shape[1], q.dtype))
+        batch, n_groups, max_group, hq, hkv, head_dim, block_tables.shape[1], q.dtype,
+        scales[0] is not None))
     _abi.call("ivakv_prefix_decode_attn", q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), *scales,
               block_tables.data_ptr(), context_lens.data_ptr(), group_start.data_ptr(),
               prefix_lens.data_ptr(), n_groups, out.data_ptr(), workspace.data_ptr(),

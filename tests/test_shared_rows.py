@@ -64,11 +64,11 @@ def test_row_workspace_sizes(iva):
     a = iva._abi
     n = ctypes.c_size_t(7)
     for name in ("ivakv_cross_workspace_size", "ivakv_prefix_workspace_size"):
-        assert call(iva, name, 2, 8, 4, 8, 2, 100, 9, a.F16, ctypes.byref(n)) == a.E_SHAPE and n.value == 0
-        assert call(iva, name, 2, 8, 4, 8, 2, 128, 9, 9, ctypes.byref(n)) == a.E_DTYPE
-        assert call(iva, name, 2, 8, 4, 8, 2, 128, 9, a.F16, None) == a.E_ARG
-        assert call(iva, name, 2, 8, 4, 8, 3, 128, 9, a.F16, ctypes.byref(n)) == a.E_SHAPE
-    assert call(iva, "ivakv_prefix_workspace_size", 2, 1, 2, 8, 2, 128, -1, a.F16, ctypes.byref(n)) == a.E_ARG
+        assert call(iva, name, 2, 8, 4, 8, 2, 100, 9, a.F16, 0, ctypes.byref(n)) == a.E_SHAPE and n.value == 0
+        assert call(iva, name, 2, 8, 4, 8, 2, 128, 9, 9, 0, ctypes.byref(n)) == a.E_DTYPE
+        assert call(iva, name, 2, 8, 4, 8, 2, 128, 9, a.F16, 0, None) == a.E_ARG
+        assert call(iva, name, 2, 8, 4, 8, 3, 128, 9, a.F16, 0, ctypes.byref(n)) == a.E_SHAPE
+    assert call(iva, "ivakv_prefix_workspace_size", 2, 1, 2, 8, 2, 128, -1, a.F16, 0, ctypes.byref(n)) == a.E_ARG
     # grows with nothing but the launch: no rows, no partials
     assert iva.cross_workspace_bytes(0, 0, 0, 8, 2, 128, 100, torch.float16) == 0
     assert iva.prefix_workspace_bytes(0, 0, 0, 8, 2, 128, 100, torch.float16) == 0

@@ -366,3 +366,22 @@ def test_row_ops_device_refusals(iva, dev):
     ws = torch.full((n + 256,), 0x7F, dtype=torch.uint8, device=dev)
     x.check(cross(iva, dev, x, workspace=ws[:n], max_query_len=2), cross_ref(x), "own workspace")
     assert (ws[n:] == 0x7F).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("d,rows,keys", [(128, [70, 65, 130], [333, 0, 200]), (256, [40, 1, 33], [130, 300, 17])])
+def test_cross_many_rows(iva, dev, dtype, d, rows, keys):
+    """Enough whole row chunks to be walked through LDS (32 kv heads), with an invalid page, a sequence
+    without keys and rows past the last whole chunk."""
+    c = cross_case(iva, dev, rows + [64] * 8, keys + [40] * 8, 128, 32, d, dtype, seed=20, holes=[(0, 3)])
+    c.check(cross(iva, dev, c), cross_ref(c), f"{dtype} D={d}")
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+def test_prefix_many_rows(iva, dev, dtype):
+    """A prefix of pieces walked through LDS: 320 rows per kv head on a wide table, rows that take
+    part and rows that do not, a ragged second group."""
+    groups = [(1000, [i % 23 for i in range(78)] + [-500, -1000]), (333, [3] * 21)]
+    c = prefix_case(iva, dev, groups, 4, 1, 128, dtype, seed=21, width=1100)
+    c.check(prefix(iva, dev, c), prefix_ref(c), str(dtype))
+    c.check(prefix(iva, dev, c, window=1005, n_sink=3), prefix_ref(c, window=1005, n_sink=3), "window")
