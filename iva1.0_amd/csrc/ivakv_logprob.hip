@@ -9,14 +9,21 @@
 // W to e^(m - m') (W + (m - m') S).  The differences z - m are exact to fp32, so a large
 // common offset of the logits costs no accuracy.
 //
-// Top k: a wave keeps its k best in one register per lane, sorted by (value, -index) and lane i
-// the i-th.  A block of a wave's elements (64 lanes x 64, in registers for the sums anyway) is
-// searched only where a lane's maximum can pass the k-th; before the list is full the bound is the k-th
-// largest of the 64 lanes' maxima, found bit by bit with ballots, so that about k elements are
-// inserted instead of all.  The waves' lists meet in LDS, where every entry finds its rank by a
-// binary search in each other list (keys are unique, so ranks are).
+// Top k, by keys (value, -index), which are unique.  The lanes' maxima bound the k-th key from
+// below: by the k-th largest of one wave's maxima, and by the least over the W waves of their
+// ceil(k / W)-th largest, found bit by bit with ballots.  A row of one block is still in registers
+// then; of a longer one only the blocks of a lane whose maximum reaches the bound are read again.
+// The few vectors with a logit that reaches the bound are listed in LDS, then their logits, and
+// there each logit counts those above it.  Where too many reach it (a constant row, say), every
+// wave keeps its k best in one register per lane, sorted, inserts what passes the k-th, and the
+// waves' lists meet in LDS, where every entry finds its rank by a binary search in each other
+// list.  (Looking for single logits among the registers at once, 64 unrolled tests, was slower:
+// 15.0 us against 11.5 at 4 rows of 32000, bf16, top 20, for the code that each wave had to fetch.)
 //
-// Bound: reading the logits once (forward), and again with one write (backward).
+// Bound: reading the logits once (forward), and again with one write (backward).  8192 rows of
+// 32000, bf16: 83 us without tops (6.3 TB/s), 130 us with the top 5; 512 rows of 131072, fp32: 45
+// and 53 us; a row of 32000: 6 us without tops, 11 us with 20 (two launches' length, most of it
+// the latencies of the load, the bound, the barriers and the lists).
 #include "ivakv_tile.h"
 
 namespace ivakv {
@@ -72,6 +79,7 @@ template <>
 struct Elem<IVAKV_F32> {
   using T = float;
   static constexpr int kVec = 4;
+  static constexpr int kKeyBits = 24;  // of a sort key that bound the tops
   static IVAKV_INLINE __device__ inline float at(const Chunk16& c, int j) { return __uint_as_float(c.w[j]); }
   static __device__ inline float one(const float* p) { return *p; }
 };
@@ -79,6 +87,7 @@ template <>
 struct Elem<IVAKV_F16> {
   using T = _Float16;
   static constexpr int kVec = 8;
+  static constexpr int kKeyBits = 19;
   static IVAKV_INLINE __device__ inline float at(const Chunk16& c, int j) {
     return (float)__builtin_bit_cast(f16x2, c.w[j >> 1])[j & 1];
   }
@@ -88,6 +97,7 @@ template <>
 struct Elem<IVAKV_BF16> {
   using T = __bf16;
   static constexpr int kVec = 8;
+  static constexpr int kKeyBits = 16;
   static IVAKV_INLINE __device__ inline float at(const Chunk16& c, int j) {
     return __uint_as_float(j & 1 ? c.w[j >> 1] & 0xFFFF0000u : c.w[j >> 1] << 16);
   }
@@ -100,6 +110,11 @@ __device__ inline uint32_t key_of(float z) {
   const uint32_t u = __float_as_uint(z + 0.f);
   if (z != z) return 0xFFFFFFFFu;
   return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+// The value of the lane below (lane 0: any).
+__device__ inline uint32_t from_lane_below(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x138, 0xF, 0xF, false);
 }
 
 // A wave's k best: lane i < k the i-th.
@@ -115,7 +130,7 @@ struct TopList {
   }
   __device__ inline void insert(uint32_t k, uint32_t i, int top, int lane) {  // (k, i) uniform
     const int p = __popcll(__builtin_amdgcn_ballot_w64(beats(key, idx, k, i)));
-    const uint32_t up_k = __shfl_up(key, 1), up_i = __shfl_up(idx, 1);
+    const uint32_t up_k = from_lane_below(key), up_i = from_lane_below(idx);
     key = lane > p ? up_k : lane == p ? k : key;
     idx = lane > p ? up_i : lane == p ? i : idx;
     kth_key = __builtin_amdgcn_readlane(key, top - 1);
@@ -133,14 +148,17 @@ struct TopList {
   }
 };
 
-// The k-th largest of the lanes' keys, or 0 when fewer than k lanes hold one.
-__device__ inline uint32_t kth_of_lanes(uint32_t key, int top) {
-  uint32_t t = 0;
-  for (int bit = 31; bit >= 0; --bit) {
-    const uint32_t c = t | (1u << bit);
-    if (__popcll(__builtin_amdgcn_ballot_w64(key >= c)) >= top) t = c;
+// The k-th and the j-th largest of the lanes' keys to BITS bits, rounded down, or 0 when fewer
+// lanes hold one.
+template <int BITS>
+__device__ inline void kth_of_lanes(uint32_t key, int k, int j, uint32_t& kth, uint32_t& jth) {
+  kth = jth = 0;
+#pragma unroll 4
+  for (int bit = 31; bit > 31 - BITS; --bit) {
+    const uint32_t c = kth | (1u << bit), d = jth | (1u << bit);
+    if (__popcll(__builtin_amdgcn_ballot_w64(key >= c)) >= k) kth = c;
+    if (__popcll(__builtin_amdgcn_ballot_w64(key >= d)) >= j) jth = d;
   }
-  return t;
 }
 
 // The entries of a sorted list of `top` in LDS that beat (k, i).
@@ -158,76 +176,75 @@ __device__ inline float value_of(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key);
 }
 
+constexpr int kCandidates = 512;
+constexpr int kMaxBlocks = 16;  // blocks of a row whose lanes' maxima are kept
+
 // One workgroup of W waves per row.
 template <int DT, bool kTop, int W>
 __global__ __launch_bounds__(64 * W) void logprob_kernel(LogprobArgs a) {
   using El = Elem<DT>;
   using T = typename El::T;
-  constexpr int VEC = El::kVec, STEPS = 8;
-  constexpr int kSpan = 64 * VEC;  // elements of a wave's load
+  constexpr int VEC = El::kVec, STEPS = 8, kThreads = 64 * W;
   __shared__ float s_m[W], s_s[W], s_w[W];
-  __shared__ uint32_t s_key[kTop ? W * kMaxTop : 1], s_idx[kTop ? W * kMaxTop : 1];
+  __shared__ float s_bmax[kTop ? kMaxBlocks : 1][kTop ? kThreads : 1];
+  __shared__ uint32_t s_key[kTop ? kCandidates : 1], s_idx[kTop ? kCandidates : 1];  // candidates, or W lists
+  static_assert(W * kMaxTop <= kCandidates, "the waves' lists fit");
+  __shared__ int s_hit[kTop ? kCandidates : 1];  // vectors that hold candidates
+  __shared__ uint32_t s_kth[W], s_least[W], s_n, s_hits;
   const int64_t row = blockIdx.x;
   const T* z = static_cast<const T*>(a.logits) + row * a.stride;
-  const int V = a.vocab;
-  const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6);
+  const int V = a.vocab, tid = threadIdx.x;
+  const int lane = tid & 63, wave = uni(tid >> 6);
   // Elements before the first 16-byte boundary and after the last are taken one by one.
   const int head = min(V, (int)((16 - ((uintptr_t)z & 15)) & 15) / (int)sizeof(T));
   const int vecs = (V - head) / VEC, tail = head + vecs * VEC;
   const Chunk16* zv = reinterpret_cast<const Chunk16*>(z + head);
+  if (kTop && tid == 0) s_n = s_hits = 0;
+  // A block: STEPS vectors per lane, the threads' loads side by side.
+  constexpr int kBlock = STEPS * kThreads;
+  const int blocks = (vecs + kBlock - 1) / kBlock;
+  auto vec_at = [&](int v0, int i) IVAKV_INLINE -> int { return v0 + i * kThreads + tid; };
   Moments mo{kLowest, 0.f, 0.f};
-  TopList list;
-  list.reset();
-  // Vectors of a wave's block: block b of the row is wave b % W's b / W-th.
-  constexpr int kBlock = 64 * STEPS;
-  for (int v0 = wave * kBlock; v0 < vecs; v0 += W * kBlock) {
-    Chunk16 c[STEPS];
+  Chunk16 c[STEPS];
+  float mx = kNegInf;  // of this lane's logits
+  for (int b = 0; b < blocks; ++b) {
+    const int v0 = b * kBlock;
 #pragma unroll
-    for (int i = 0; i < STEPS; ++i) c[i] = load_nt<Chunk16>(zv + min(v0 + 64 * i + lane, vecs - 1));
-    float smax[STEPS], mx = kNegInf;
+    for (int i = 0; i < STEPS; ++i) c[i] = load_nt<Chunk16>(zv + min(vec_at(v0, i), vecs - 1));
+    float bm = kNegInf;
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) {
       float t = El::at(c[i], 0);
 #pragma unroll
       for (int j = 1; j < VEC; ++j) t = fmaxf(t, El::at(c[i], j));
-      smax[i] = v0 + 64 * i + lane < vecs ? t : kNegInf;
-      mx = fmaxf(mx, smax[i]);
+      bm = fmaxf(bm, vec_at(v0, i) < vecs ? t : kNegInf);
     }
-    mo.to_max(fmaxf(mo.m, mx));
+    if constexpr (kTop)
+      if (b < kMaxBlocks) s_bmax[b][tid] = bm;
+    mx = fmaxf(mx, bm);
+    mo.to_max(fmaxf(mo.m, bm));
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) {
-      if (v0 + 64 * i + lane < vecs) {
+      if (vec_at(v0, i) < vecs) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) mo.add(El::at(c[i], j));
       }
     }
-    if constexpr (kTop) {
-      // fmaxf drops a NaN, which leads the order: such rows are searched without a bound
-      const bool nan = mo.s != mo.s;
-      const bool any_nan = __builtin_amdgcn_ballot_w64(nan) != 0;
-      uint32_t bound = list.kth_key;
-      if (bound == 0 && !any_nan) bound = kth_of_lanes(v0 + lane < vecs ? key_of(mx) : 0u, a.top);
-#pragma unroll
-      for (int i = 0; i < STEPS; ++i) {
-        const bool in = v0 + 64 * i + lane < vecs;
-        if (!any_nan && __builtin_amdgcn_ballot_w64(in && key_of(smax[i]) >= bound) == 0) continue;
-        const int at = head + (v0 + 64 * i + lane) * VEC;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const uint32_t k = key_of(El::at(c[i], j));
-          list.offer(in && k >= bound, k, (uint32_t)(at + j), a.top, lane);
-        }
-        bound = max(bound, list.kth_key);
-      }
-    }
   }
-  if (wave == 0) {  // the row's ends: at most VEC - 1 elements each
-    const int e = lane < head ? lane : tail + (lane - head);
-    const bool in = lane < head || e < V;
-    const float x = in ? El::one(z + e) : kNegInf;
-    mo.to_max(fmaxf(mo.m, x));
-    if (in) mo.add(x);
-    if constexpr (kTop) list.offer(in, key_of(x), (uint32_t)e, a.top, lane);
+  // The row's ends, on wave 0: at most VEC - 1 elements each.
+  const int e_at = lane < head ? lane : tail + (lane - head);
+  const bool e_in = wave == 0 && (lane < head || e_at < V);
+  const float e_x = e_in ? El::one(z + e_at) : kNegInf;
+  mo.to_max(fmaxf(mo.m, e_x));
+  if (e_in) mo.add(e_x);
+  if constexpr (kTop) {
+    const uint32_t mine = e_in || tid < vecs ? key_of(fmaxf(mx, e_x)) : 0u;
+    uint32_t kth, least;
+    kth_of_lanes<El::kKeyBits>(mine, a.top, (a.top + W - 1) / W, kth, least);
+    if (lane == 0) {
+      s_kth[wave] = kth;
+      s_least[wave] = least;
+    }
   }
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1)
@@ -237,12 +254,6 @@ __global__ __launch_bounds__(64 * W) void logprob_kernel(LogprobArgs a) {
     s_s[wave] = mo.s;
     s_w[wave] = mo.w;
   }
-  if constexpr (kTop) {
-    if (lane < a.top) {
-      s_key[wave * kMaxTop + lane] = list.key;
-      s_idx[wave * kMaxTop + lane] = list.idx;
-    }
-  }
   __syncthreads();
   Moments all{s_m[0], s_s[0], s_w[0]};
 #pragma unroll
@@ -250,7 +261,7 @@ __global__ __launch_bounds__(64 * W) void logprob_kernel(LogprobArgs a) {
   // No finite logit: no distribution; log probabilities -inf, entropy 0.
   const bool none = all.s == 0.f;
   const float log_s = none ? 0.f : logf(all.s);
-  if (threadIdx.x == 0) {
+  if (tid == 0) {
     const int64_t t = a.tokens[row];
     const bool given = t >= 0 && t < V;
     a.logprobs[row] = given ? (El::one(z + (given ? t : 0)) - all.m) - log_s : 0.f;
@@ -261,18 +272,114 @@ __global__ __launch_bounds__(64 * W) void logprob_kernel(LogprobArgs a) {
     }
   }
   if constexpr (kTop) {
-    for (int e = threadIdx.x; e < W * a.top; e += 64 * W) {
+    auto emit = [&](int rank, uint32_t k, uint32_t i) IVAKV_INLINE {
+      if (rank >= a.top) return;
+      a.top_logprobs[row * a.top + rank] = (value_of(k) - all.m) - log_s;
+      a.top_tokens[row * a.top + rank] = i;
+    };
+    uint32_t bound = s_kth[0], least = s_least[0];
+#pragma unroll
+    for (int u = 1; u < W; ++u) {
+      bound = max(bound, s_kth[u]);
+      least = min(least, s_least[u]);
+    }
+    bound = max(bound, least);
+    const bool nan = all.s != all.s;  // (the maxima drop a NaN: such a row is searched whole)
+    auto gather = [&](float x, int at) IVAKV_INLINE {
+      const uint32_t k = key_of(x);
+      if (k >= bound) {
+        const uint32_t n = atomicAdd(&s_n, 1u);
+        if (n < kCandidates) {
+          s_key[n] = k;
+          s_idx[n] = (uint32_t)at;
+        }
+      }
+    };
+    auto hits_of = [&](int v0) IVAKV_INLINE {
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i) {
+        float t = El::at(c[i], 0);
+#pragma unroll
+        for (int j = 1; j < VEC; ++j) t = fmaxf(t, El::at(c[i], j));
+        const int v = vec_at(v0, i);
+        if (v < vecs && (nan || key_of(t) >= bound)) {
+          const uint32_t n = atomicAdd(&s_hits, 1u);
+          if (n < kCandidates) s_hit[n] = v;
+        }
+      }
+    };
+    if (blocks <= kMaxBlocks) {
+      if (blocks == 1) {
+        if (nan || key_of(mx) >= bound) hits_of(0);
+      } else {
+        for (int b = 0; b < blocks; ++b) {
+          if (!nan && key_of(s_bmax[b][tid]) < bound) continue;
+#pragma unroll
+          for (int i = 0; i < STEPS; ++i) c[i] = zv[min(vec_at(b * kBlock, i), vecs - 1)];
+          hits_of(b * kBlock);
+        }
+      }
+      __syncthreads();
+      const int hits = (int)s_hits;
+      if (hits <= kCandidates) {
+        for (int e = tid; e < hits * VEC; e += kThreads) {
+          const int at = head + s_hit[e / VEC] * VEC + e % VEC;
+          gather(El::one(z + at), at);
+        }
+        if (e_in) gather(e_x, e_at);
+      }
+      __syncthreads();
+      const int n = hits <= kCandidates ? (int)s_n : hits;
+      if (n <= kCandidates) {
+        // Every wave holds the candidates, 64 to a register, and ranks each W-th.
+        constexpr int M = kCandidates / 64;
+        uint32_t ck[M], ci[M];
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+          const bool in = 64 * m + lane < n;
+          ck[m] = in ? s_key[64 * m + lane] : 0u;
+          ci[m] = in ? s_idx[64 * m + lane] : 0u;
+        }
+        for (int e = wave; e < n; e += W) {
+          const uint32_t k = s_key[e], i = s_idx[e];
+          int rank = 0;
+#pragma unroll
+          for (int m = 0; m < M; ++m)
+            if (64 * m < n) rank += __popcll(__builtin_amdgcn_ballot_w64(TopList::beats(ck[m], ci[m], k, i)));
+          if (lane == 0) emit(rank, k, i);
+        }
+        return;
+      }
+      __syncthreads();
+    }
+    TopList list;
+    list.reset();
+    for (int b = 0; b < blocks; ++b) {
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i) {
+        const int v = vec_at(b * kBlock, i);
+        const Chunk16 x = zv[min(v, vecs - 1)];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const uint32_t k = key_of(El::at(x, j));
+          list.offer(v < vecs && k >= bound, k, (uint32_t)(head + v * VEC + j), a.top, lane);
+        }
+      }
+    }
+    list.offer(e_in, key_of(e_x), (uint32_t)e_at, a.top, lane);
+    if (lane < a.top) {
+      s_key[wave * kMaxTop + lane] = list.key;
+      s_idx[wave * kMaxTop + lane] = list.idx;
+    }
+    __syncthreads();
+    for (int e = tid; e < W * a.top; e += kThreads) {
       const int u = e / a.top, at = e % a.top;
       const uint32_t k = s_key[u * kMaxTop + at], i = s_idx[u * kMaxTop + at];
       if (k == 0) continue;  // an empty place
       int rank = at;
-#pragma unroll
       for (int o = 0; o < W; ++o)
         if (o != u) rank += beating(s_key + o * kMaxTop, s_idx + o * kMaxTop, a.top, k, i);
-      if (rank < a.top) {
-        a.top_logprobs[row * a.top + rank] = (value_of(k) - all.m) - log_s;
-        a.top_tokens[row * a.top + rank] = i;
-      }
+      emit(rank, k, i);
     }
   }
 }
@@ -357,9 +464,17 @@ int check_logits(const char* name, const void* logits, int64_t stride, int64_t n
   return IVAKV_OK;
 }
 
+// Waves of a row: one where one holds it in its registers (8192 rows of 512, bf16, top 5: 19 us;
+// four waves 47); eight for few rows, whose time is latency (4 rows of 131072, fp32, top 20: 27 us
+// against 37; 512 rows of 32000, bf16: 18 against 20); else four (1024 rows: 27 us against 30;
+// 8192: 130 against 163).
+constexpr int kFewRows = 512;
+
 template <int DT, bool kTop>
 void launch_logprob(const LogprobArgs& a, hipStream_t stream) {
-  logprob_kernel<DT, kTop, 4><<<(unsigned)a.n, 256, 0, stream>>>(a);
+  if (a.vocab <= 512 * Elem<DT>::kVec) logprob_kernel<DT, kTop, 1><<<(unsigned)a.n, 64, 0, stream>>>(a);
+  else if (a.n <= kFewRows) logprob_kernel<DT, kTop, 8><<<(unsigned)a.n, 512, 0, stream>>>(a);
+  else logprob_kernel<DT, kTop, 4><<<(unsigned)a.n, 256, 0, stream>>>(a);
 }
 
 template <int DT>
