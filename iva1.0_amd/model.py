@@ -473,20 +473,34 @@ class AttentionTorch(_AttentionBase):
         return self.o_proj(out), kv_cache
 
 
-# Bytes of K and V per layer that forked sequences would read again, from which a decode step
-# appends and attends through the shared prefix instead of in the one fused step.
-SHARED_MIN_BYTES = 32 << 20
+# A decode step of forked sequences reads the pages they share once where that saves at least
+# SHARED_MIN_BYTES of K and V per layer, in prefixes of SHARED_MIN_TOKENS or more: attention of a
+# layer on the GPU, fused append and decode : append and shared prefix, bf16, 32 heads over 8 of
+# 128, 8 sequences of 1024 + 64 tokens (28 MiB saved) 16.0 : 16.7 us, of 2048 + 64 (56) 19.1 : 17.6;
+# 16 of 1024 (60) 21.1 : 18.5; 32 of 1024 + 300 (124) 27.8 : 23.7; but a short prefix stays in the
+# caches by itself, 32 of 512 + 100 (62) 12.9 : 19.4, 64 of 512 + 300 (126) 25.5 : 31.8.  A whole
+# layer of d_model 4096 in a replayed graph, 32 of 2048 tokens (248) 226 : 210, 64 of 4096 (1008)
+# 295 : 213; of d_model 1024 75 : 61 and 200 : 114.
+# Called one by one, a narrow layer is bound by the host, to which the fused step is one call: d_model
+# 1024, 16 of 8192 tokens (480 MiB) 88 : 114, 64 of 4096 (1008) 272 : 292, and of d_model 4096, which
+# is not, 213 : 177 and 296 : 293.  There it has to save SHARED_EAGER times as much.
+SHARED_MIN_BYTES = 56 << 20
+SHARED_MIN_TOKENS = 1024
+SHARED_EAGER = 16
 
 
-def _reads_shared(cache: Any, window: Optional[int]) -> bool:
+def _reads_shared(cache: Any, window: Optional[int], d_model: int) -> bool:
     """A paged cache whose forked sequences share enough for paged_prefix_decode_attention, and
     see all of it."""
     shared = getattr(cache, "shared", None)
     if shared is None or (window and 0 < window <= cache.seq_len):
         return False
     pool = cache.pool
-    row = 2 * pool.num_kv_heads * pool.head_dim * pool.dtype.itemsize
-    return shared.saved_tokens * row >= SHARED_MIN_BYTES
+    saved = shared.saved_tokens * 2 * pool.num_kv_heads * pool.head_dim * pool.dtype.itemsize
+    if saved < SHARED_MIN_BYTES or shared.shortest < SHARED_MIN_TOKENS:
+        return False
+    return (d_model >= 4096 or saved >= SHARED_EAGER * SHARED_MIN_BYTES
+            or torch.cuda.is_current_stream_capturing())
 
 
 class PagedAttention(_AttentionBase):
@@ -536,7 +550,7 @@ class PagedAttention(_AttentionBase):
         paged cache of 16-bit pages like x or FP8 pages, causal, without mask or RoPE."""
         if (attention_mask is not None or type(cache) is not PagedKVCache or x.shape[1] != 1
                 or not self.causal or self.rope or (self.training and self.dropout > 0)
-                or _reads_shared(cache, window)):
+                or _reads_shared(cache, window, self.d_model)):
             return False
         pool = cache.pool
         return ((pool.dtype is x.dtype or pool.fp8) and pool.num_kv_heads == self.n_kv_heads
@@ -608,7 +622,7 @@ class PagedAttention(_AttentionBase):
             # (ivakv_gather) by the kernels, and the masked attention evaluated on the
             # gathered keys in torch (the paged attention kernels take no per-key mask)
             decode = s == 1 and self.causal and key_ok is None
-            shared_prefix = decode and _reads_shared(kv_cache, window)
+            shared_prefix = decode and _reads_shared(kv_cache, window, self.d_model)
             fp8 = kv_cache.pool.fp8
             view = kv_cache.layer_step(k.contiguous(), v.contiguous(), append=not decode,
                                        rope_positions=rope_pos, rope_theta=self.rope_theta)

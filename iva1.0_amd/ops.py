@@ -827,6 +827,9 @@ def prefix_workspace_bytes(batch: int, n_groups: int, max_group: int, num_q_head
                                 int(head_dim), int(max_blocks), dtype_code(dtype), int(fp8))
 
 
+MAX_PREFIX_ROWS = 8192  # of one paged_prefix_decode_attention call
+
+
 def paged_prefix_decode_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
                                   block_tables: torch.Tensor, context_lens: torch.Tensor,
                                   group_start: torch.Tensor, prefix_lens: torch.Tensor,
@@ -847,7 +850,7 @@ def paged_prefix_decode_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool:
     the attention tolerance.  ``max_group`` (>= the largest group's rows) sizes the launch; when
     omitted it is read back from ``group_start`` (a device sync), which is then checked.
     ``workspace`` (:func:`prefix_workspace_bytes`) is kept per device and stream when omitted.  At
-    most 8192 rows.
+    most MAX_PREFIX_ROWS rows, with less than 2^31 entries of ``block_tables`` times KV heads.
 
     Replaces the cache branch of ``AttentionTorch.forward`` (src/core/attention.py:77-102).
     """

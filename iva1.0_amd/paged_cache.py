@@ -31,7 +31,8 @@ from typing import Dict, List, Optional, Sequence, Tuple
 import numpy as np
 import torch
 
-from .ops import FP8, chunk_slots, copy_pages, kv_append, kv_gather, pool_shapes, scale_shape
+from .ops import (FP8, MAX_PREFIX_ROWS, chunk_slots, copy_pages, kv_append, kv_gather, pool_shapes,
+                  scale_shape)
 
 
 class OutOfPagesError(RuntimeError):
@@ -436,10 +437,7 @@ class SharedPrefix:
     prefix_lens: torch.Tensor   # int32 [n_groups], whole pages
     max_group: int
     saved_tokens: int           # tokens of K and V per layer that sharing need not read again
-
-    @property
-    def op_args(self) -> tuple:
-        return self.group_start, self.prefix_lens
+    shortest: int               # of the prefixes
 
 
 @dataclass
@@ -641,11 +639,13 @@ class PagedKVCache:
         self._shared_tokens = self.seq_len // self.block_size * self.block_size
         self._bt_gen = -1
         self.shared = None
-        if self._shared_tokens:
+        # (more sequences than paged_prefix_decode_attention takes decode one by one)
+        if (self._shared_tokens and self.batch_size <= MAX_PREFIX_ROWS
+                and self.batch_size * self.pool.max_blocks * self.pool.num_kv_heads < 2 ** 31):
             on = dict(dtype=torch.int32, device=self.device)
             self.shared = SharedPrefix(torch.arange(0, self.batch_size + 1, n, **on),
                                        torch.full((before,), self._shared_tokens, **on), n,
-                                       before * (n - 1) * self._shared_tokens)
+                                       before * (n - 1) * self._shared_tokens, self._shared_tokens)
 
     def free(self) -> None:
         """Returns every page of this cache's sequences to the pool."""

@@ -46,6 +46,29 @@ def test_cache_fork_shares_pages(P):
     assert c.pool.num_free_pages == 40
 
 
+def test_more_rows_than_the_shared_op_takes_are_not_grouped(P, monkeypatch):
+    monkeypatch.setattr(P, "MAX_PREFIX_ROWS", 5)
+    c = cache_of(P, 2, 37, max_seqs=6, num_pages=40)
+    c.fork(3)
+    assert c.batch_size == 6 and c.shared is None
+
+
+def test_a_decode_step_reads_shared_pages_where_that_pays(P, M):
+    """By the bytes saved, the prefix, the window and the width."""
+    from types import SimpleNamespace as NS
+    pool = NS(num_kv_heads=8, head_dim=128, dtype=torch.bfloat16)  # 4 KiB a token
+    def cache(saved, shortest):
+        return NS(seq_len=3000, pool=pool, shared=P.SharedPrefix(None, None, 8, saved, shortest))
+    assert M._reads_shared(cache(7 * 2048, 2048), None, 4096)
+    assert not M._reads_shared(cache(7 * 2048 - 1, 2048), None, 4096)
+    assert not M._reads_shared(cache(31 * 512, 512), None, 4096)
+    assert not M._reads_shared(cache(7 * 2048, 2048), 3000, 4096)
+    assert M._reads_shared(cache(7 * 2048, 2048), 3001, 4096)
+    assert M._reads_shared(cache(16 * 7 * 2048, 2048), None, 1024)
+    assert not M._reads_shared(NS(seq_len=3000, pool=pool, shared=None), None, 4096)
+    assert not M._reads_shared(None, None, 4096)
+
+
 def test_cache_fork_of_a_short_or_whole_prompt(P):
     short = cache_of(P, 1, 9, max_seqs=4, num_pages=8)
     short.fork(4)
@@ -53,6 +76,7 @@ def test_cache_fork_of_a_short_or_whole_prompt(P):
     whole = cache_of(P, 1, 32, max_seqs=2, num_pages=2)
     whole.fork(2)  # no partial page: no page is needed
     assert whole.shared.prefix_lens.tolist() == [32] and whole.pool.num_free_pages == 0
+    assert whole.shared.shortest == 32
     one = cache_of(P, 1, 20)
     one.fork(1)
     assert one.shared is None and one.batch_size == 1

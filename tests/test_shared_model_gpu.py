@@ -32,6 +32,7 @@ def test_forked_decode_equals_separate_sequences(M, dev, monkeypatch, kw):
     """Two prompts, three samples each, ten different tokens: through the shared pages, and as
     six separate sequences without sharing."""
     monkeypatch.setattr(M, "SHARED_MIN_BYTES", 0)
+    monkeypatch.setattr(M, "SHARED_MIN_TOKENS", 0)
     model = model_of(M, dev, **kw)
     gen = torch.Generator().manual_seed(1)
     prompt = torch.randint(0, 512, (2, 83), generator=gen).to(dev)
@@ -58,6 +59,7 @@ def test_generate_samples_and_logprobs(M, dev, monkeypatch, use_graph):
     scoring pass over the generated sequence; shared pages taken and not."""
     model = model_of(M, dev, dtype=torch.float16)
     ids = torch.randint(0, 512, (2, 50), generator=torch.Generator().manual_seed(2)).to(dev)
+    monkeypatch.setattr(M, "SHARED_MIN_TOKENS", 0)
     for least in (0, 1 << 60):
         monkeypatch.setattr(M, "SHARED_MIN_BYTES", least)
         tokens, found = model.generate(ids, max_length=12, do_sample=False, eos_token_id=None, num_samples=3,
