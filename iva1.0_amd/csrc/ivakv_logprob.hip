@@ -22,8 +22,8 @@
 //
 // Bound: reading the logits once (forward), and again with one write (backward).  8192 rows of
 // 32000, bf16: 83 us without tops (6.3 TB/s), 130 us with the top 5; 512 rows of 131072, fp32: 45
-// and 53 us; a row of 32000: 6 us without tops, 11 us with 20 (two launches' length, most of it
-// the latencies of the load, the bound, the barriers and the lists).
+// and 53 us; a row of 32000: 6 us without tops, 11 us with 20, the latencies of the load, the
+// bound, the barriers and the lists.  Both passes of 4096 rows of 32000, bf16: 131 us.
 #include "ivakv_tile.h"
 
 namespace ivakv {
@@ -209,8 +209,15 @@ __global__ __launch_bounds__(64 * W) void logprob_kernel(LogprobArgs a) {
   float mx = kNegInf;  // of this lane's logits
   for (int b = 0; b < blocks; ++b) {
     const int v0 = b * kBlock;
+    // A backward pass reads the row again: then it is left in the caches (4096 rows of 32000, bf16,
+    // both passes 131 us against 149; the forward pass alone is faster past them, 83 against 94).
+    if (a.stats) {
 #pragma unroll
-    for (int i = 0; i < STEPS; ++i) c[i] = load_nt<Chunk16>(zv + min(vec_at(v0, i), vecs - 1));
+      for (int i = 0; i < STEPS; ++i) c[i] = zv[min(vec_at(v0, i), vecs - 1)];
+    } else {
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i) c[i] = load_nt<Chunk16>(zv + min(vec_at(v0, i), vecs - 1));
+    }
     float bm = kNegInf;
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) {
