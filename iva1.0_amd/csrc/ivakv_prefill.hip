@@ -1076,8 +1076,8 @@ __global__ __launch_bounds__((PrefillShape<DT, D, true>::kThreads)) void rows_wi
   if ((int)blockIdx.x >= n_wg) return;
   const int wg = (int)xcd_contiguous_block(blockIdx.x, n_wg);
   Group group;
-  int g, piece, h, chunk;
-  if (!pc.find(a, own, wg, lane, group, g, piece, h, chunk)) return;
+  int g, piece, h, chunk, slot;
+  if (!pc.find(a, own, wg, lane, group, g, piece, h, chunk, slot)) return;
   const int table = a.prefix ? prefix_row(a, group.pages, group.r0, group.r1, lane) : g;
   if (table < 0) return;
   RowBlock blk;
@@ -1106,7 +1106,7 @@ __global__ __launch_bounds__((PrefillShape<DT, D, true>::kThreads)) void rows_wi
   const bool whole = !a.prefix && pc.of(group) == 1;
   const int lo = piece * (pc.len / 2);
   prefill_rows<DT, D, false, true, false>(p, bt, blk, table, h, lo, min(lo + pc.len / 2, blk.n_pairs),
-                                          whole ? -1 : wg);
+                                          whole ? -1 : slot);
 }
 
 template <int DT, int D>

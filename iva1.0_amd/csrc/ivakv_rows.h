@@ -95,10 +95,13 @@ __device__ inline int wave_sum(int x) { return __builtin_amdgcn_readlane(wave_sc
 // workgroup's waves take at once), the shortest of four lengths with which all groups' items, pieces
 // times row chunks, number at most a.items.  The last of the four, sum (pages x chunks) / (items -
 // sum chunks), always does: a group has at most one piece that is not whole.  Without a.split
-// every group is one piece.  Partials, and the shared workgroups, are numbered group by group, in it
-// piece by piece, kv head by kv head, chunk by chunk.  A cross group without keys has one empty
-// piece, which writes its rows' zeros.  Each wave works this out for itself, 64 groups at a time,
-// the first 64 (`own`, group `lane`) from registers.
+// every group is one piece.  Partials are numbered group by group, in it piece by piece, kv head by kv
+// head, chunk by chunk; the shared workgroups kv head by kv head, so that an XCD, which takes a
+// contiguous run of them, gets its share of every group, long or short (bf16, 16 sequences of 97 .. 448
+// rows on 700 .. 1500 keys, 16 heads of 64: 44 us against 51 group by group; 32 / 8 heads of 128 on FP8
+// pages 186 against 204; 64 FP8 rows behind one prefix 54.8 against 53.8).  A cross group without keys
+// has one empty piece, which writes its rows' zeros.  Each wave works this out for itself, 64 groups
+// at a time, the first 64 (`own`, group `lane`) from registers.
 struct Pieces {
   int len, least, items;  // items: of all groups
   __device__ inline int of(const Group& x) const {
@@ -133,25 +136,27 @@ struct Pieces {
     }
   }
 
-  // What shared workgroup `wg` does: the group, which of its pieces, kv head and chunk; false when
-  // there is nothing for it.
+  // What shared workgroup `wg` does: the group, which of its pieces, kv head and chunk, and its
+  // partial; false when there is nothing for it.
   __device__ inline bool find(const RowArgs& a, const Group& own, int wg, int lane, Group& group, int& g, int& piece,
-                              int& h, int& chunk) const {
+                              int& h, int& chunk, int& slot) const {
+    h = (int)((uint32_t)wg / (uint32_t)items);
+    const int item = wg - h * items;
     int before = 0;
     for (int g0 = 0; g0 < a.n_groups; g0 += 64) {
       const Group x = g0 == 0 ? own : load_group(a, g0 + lane);
-      const int n = of(x) * x.chunks * a.Hkv, incl = wave_scan(n);
-      const uint64_t has = __builtin_amdgcn_ballot_w64(wg < before + incl);
+      const int n = of(x) * x.chunks, incl = wave_scan(n);
+      const uint64_t has = __builtin_amdgcn_ballot_w64(item < before + incl);
       if (has != 0) {
         const int w = __builtin_ctzll(has);
         g = g0 + w;
         group = Group{__builtin_amdgcn_readlane(x.r0, w), __builtin_amdgcn_readlane(x.r1, w),
                       __builtin_amdgcn_readlane(x.chunks, w), __builtin_amdgcn_readlane(x.pages, w)};
-        const uint32_t at = (uint32_t)(wg - before - (__builtin_amdgcn_readlane(incl, w) - __builtin_amdgcn_readlane(n, w)));
+        const int first = before + __builtin_amdgcn_readlane(incl, w) - __builtin_amdgcn_readlane(n, w);
+        const uint32_t at = (uint32_t)(item - first);
         chunk = (int)(at % (uint32_t)group.chunks);
-        const uint32_t ph = at / (uint32_t)group.chunks;
-        h = (int)(ph % (uint32_t)a.Hkv);
-        piece = (int)(ph / (uint32_t)a.Hkv);
+        piece = (int)(at / (uint32_t)group.chunks);
+        slot = first * a.Hkv + (piece * a.Hkv + h) * group.chunks + chunk;
         return true;
       }
       before += __builtin_amdgcn_readlane(incl, 63);

@@ -557,13 +557,13 @@ __device__ inline void shared_walk(const RowArgs& a, const int32_t* __restrict__
   const Group own = load_group(a, lane);
   const Pieces pc(a, own, lane);
   // Each XCD takes a contiguous run of the workgroups, so that a piece's chunks are on one XCD, one
-  // after the other: chunks past the first find the pages in its L2.
+  // after the other (chunks past the first find the pages in its L2), and all groups of a kv head.
   const int n_wg = pc.items * a.Hkv;
   if (wg >= n_wg) return;
   wg = (int)xcd_contiguous_block(wg, n_wg);
   Group group;
-  int g, piece, h, chunk;
-  if (!pc.find(a, own, wg, lane, group, g, piece, h, chunk)) return;
+  int g, piece, h, chunk, slot;
+  if (!pc.find(a, own, wg, lane, group, g, piece, h, chunk, slot)) return;
   const int rows = min(group.r1 - group.r0, a.max_rows) * a.G;  // (at most n_rows * Hq, which the entry checks)
   KeyList kl;
   kl.num_pages = a.num_pages;
@@ -582,7 +582,6 @@ __device__ inline void shared_walk(const RowArgs& a, const int32_t* __restrict__
   join_waves<WalkT, D, NR, W>(wk, smem, wave, ln, lq, s_fin);
   const float* s_acc = smem + 2 * W * R;
   const bool whole = !a.prefix && pc.of(group) == 1;
-  const int64_t slot = wg;
   const int Hq = a.Hkv * a.G;
   for (int e = threadIdx.x; e < R * (D / 4); e += 64 * W) {
     const int row = e / (D / 4), d = 4 * (e % (D / 4)), r = chunk * R + row;
@@ -596,8 +595,8 @@ __device__ inline void shared_walk(const RowArgs& a, const int32_t* __restrict__
 #pragma unroll
       for (int i = 0; i < 4; ++i) dst[i] = WalkT::Tr::from_float(o[i] * inv);
     } else {
-      *reinterpret_cast<f32x4*>(a.part_acc + (slot * R + row) * D + d) = o;
-      if (d == 0) *reinterpret_cast<f32x2*>(a.part_ml + (slot * R + row) * 2) = f32x2{s_fin[2 * row], s_fin[2 * row + 1]};
+      *reinterpret_cast<f32x4*>(a.part_acc + ((int64_t)slot * R + row) * D + d) = o;
+      if (d == 0) *reinterpret_cast<f32x2*>(a.part_ml + ((int64_t)slot * R + row) * 2) = f32x2{s_fin[2 * row], s_fin[2 * row + 1]};
     }
   }
 }
@@ -919,9 +918,9 @@ struct Plan {
 // Whether a group's shared walk goes through LDS in chunks of up to 256 rows (wide) rather than through
 // the waves' own registers in chunks of 32.  It reads the pages from the L2 once for eight times the
 // rows, but leaves a partial of all rows per piece and has one workgroup per CU to hide a piece's
-// start and end.  So it takes cross attention where whole chunks need no cutting into pieces (fp16,
+// start and end.  So it takes cross attention where whole chunks need no cutting into pieces (bf16,
 // D 128, walk : wide in us: 8 sequences of 200 x 2000, 32 / 8 heads 105 : 79, 16 of 97 .. 448 x 700 ..
-// 1500 200 : 151; cut in two, 16 of 64 x 1000 .. 1500 57 : 73), and a prefix long for its rows (768 rows on
+// 1500 200 : 151; cut in two, 16 of 64 x 1000 .. 1500 57 : 73), and a prefix long for its rows (bf16, 768 rows on
 // 8192 tokens 81 : 69, 1024 on 16384 155 : 128; 512 on 8192 49 : 57, 1024 on 2048 47 : 58).  At head_dim
 // 64 the softmax bounds both (16 of 448 x 1500, 16 heads 79 : 87).  FP8 pages would be rounded to the
 // queries' type on the way.
