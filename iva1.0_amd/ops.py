@@ -19,6 +19,7 @@ from functools import lru_cache, partial
 from typing import Dict, List, NamedTuple, Optional, Tuple
 
 import torch
+import torch.autograd.forward_ad as fwAD
 
 from . import _abi
 
@@ -124,6 +125,8 @@ def _stream(dev: torch.device) -> int:
 def _capturing(dev: torch.device) -> bool:
     """True while the device's current stream is being captured into a HIP graph, when
     no host read of device data is allowed (the kernels' own bounds checks then stand)."""
+    if dev.index == _current_device():  # (entering a device costs the host 2 us)
+        return torch.cuda.is_current_stream_capturing()
     with torch.cuda.device(dev):
         return torch.cuda.is_current_stream_capturing()
 
@@ -893,24 +896,29 @@ class TokenLogprobs(NamedTuple):
     top_tokens: torch.Tensor     # int64 [..., top_k]
 
 
+def _token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int,
+                    stats: Optional[torch.Tensor]):
+    n, vocab = logits.shape
+    dev = logits.device
+    logprobs = torch.empty(n, dtype=torch.float32, device=dev)
+    entropy = torch.empty(n, dtype=torch.float32, device=dev)
+    top = torch.empty(n, top_k, dtype=torch.float32, device=dev)
+    top_tokens = torch.empty(n, top_k, dtype=torch.int64, device=dev)
+    _abi.call("ivakv_token_logprobs", logits.data_ptr(), logits.stride(0), tokens.data_ptr(), n,
+              vocab, top_k, logprobs.data_ptr(), entropy.data_ptr(),
+              stats.data_ptr() if stats is not None else None, top.data_ptr(), top_tokens.data_ptr(),
+              dtype_code(logits.dtype), _stream(dev))
+    return logprobs, entropy, top, top_tokens
+
+
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits: torch.Tensor, tokens: torch.Tensor, top_k: int, keep: bool):
-        n, vocab = logits.shape
-        dev = logits.device
-        logprobs = torch.empty(n, dtype=torch.float32, device=dev)
-        entropy = torch.empty(n, dtype=torch.float32, device=dev)
-        stats = torch.empty(n, 2, dtype=torch.float32, device=dev) if keep else None
-        top = torch.empty(n, top_k, dtype=torch.float32, device=dev)
-        top_tokens = torch.empty(n, top_k, dtype=torch.int64, device=dev)
-        _abi.call("ivakv_token_logprobs", logits.data_ptr(), logits.stride(0), tokens.data_ptr(), n,
-                  vocab, top_k, logprobs.data_ptr(), entropy.data_ptr(),
-                  stats.data_ptr() if keep else None, top.data_ptr(), top_tokens.data_ptr(),
-                  dtype_code(logits.dtype), _stream(dev))
-        if keep:
-            ctx.save_for_backward(logits, tokens, entropy, stats, top_tokens)
-        ctx.mark_non_differentiable(top_tokens)
-        return logprobs, entropy, top, top_tokens
+    def forward(ctx, logits: torch.Tensor, tokens: torch.Tensor, top_k: int):
+        stats = torch.empty(logits.shape[0], 2, dtype=torch.float32, device=logits.device)
+        out = _token_logprobs(logits, tokens, top_k, stats)
+        ctx.save_for_backward(logits, tokens, out[1], stats, out[3])
+        ctx.mark_non_differentiable(out[3])
+        return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -923,7 +931,7 @@ class _TokenLogprobs(torch.autograd.Function):
                   tokens.data_ptr(), entropy.data_ptr(), stats.data_ptr(), top_tokens.data_ptr(),
                   g.data_ptr(), gh.data_ptr(), gt.data_ptr(), n, vocab, top_tokens.shape[1],
                   grad.data_ptr(), dtype_code(logits.dtype), _stream(logits.device))
-        return grad, None, None, None
+        return grad, None, None
 
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0) -> TokenLogprobs:
@@ -950,16 +958,21 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0) -
     vocab, top_k = logits.shape[-1], int(top_k)
     if not 0 <= top_k <= min(vocab, MAX_TOP_LOGPROBS):
         raise ValueError(f"top_k must be in [0, {min(vocab, MAX_TOP_LOGPROBS)}], got {top_k}")
-    lead = tuple(tokens.shape)
-    rows = logits.reshape(-1, vocab) if vocab else logits.reshape(tokens.numel(), 0)
-    if rows.shape[0] and not vocab:
+    lead = tokens.shape
+    if tokens.numel() and not vocab:
         raise ValueError("rows without logits")
-    if rows.numel() and rows.stride(1) != 1:
+    rows = logits if logits.dim() == 2 else logits.reshape(tokens.numel(), vocab)
+    if rows.stride(1) != 1 and rows.numel():
         rows = rows.contiguous()
-    flat = tokens.reshape(-1).to(torch.int64).contiguous()
-    keep = torch.is_grad_enabled() and logits.requires_grad
-    lp, h, top, ids = _TokenLogprobs.apply(rows, flat, top_k, keep)
-    return TokenLogprobs(lp.view(lead), h.view(lead), top.view(*lead, top_k), ids.view(*lead, top_k))
+    flat = tokens if tokens.dim() == 1 else tokens.reshape(-1)
+    flat = flat.to(torch.int64).contiguous()
+    if (torch.is_grad_enabled() and logits.requires_grad) or fwAD._current_level >= 0:
+        out = _TokenLogprobs.apply(rows, flat, top_k)
+    else:
+        out = _token_logprobs(rows, flat, top_k, None)
+    if len(lead) != 1:
+        out = [t.view((*lead, *t.shape[1:])) for t in out]
+    return TokenLogprobs(*out)
 
 
 def rope_(x: torch.Tensor, positions: torch.Tensor, theta: float = 10000.0) -> torch.Tensor:
