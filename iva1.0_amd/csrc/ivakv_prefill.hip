@@ -1064,7 +1064,9 @@ __global__ __launch_bounds__((PrefillShape<DT, D, true>::kThreads)) void prefill
 
 // The shared walk of ivakv_rows.hip for many rows: a workgroup takes up to kRowsWG rows of a group and
 // a piece of its pages, staged through LDS once for all of them, and leaves one partial (or, where
-// cross attention does not cut, the finished rows).
+// cross attention does not cut, the finished rows).  Bound as the prefill, by instruction issue beside
+// the MFMAs: 16 sequences of 97 .. 448 rows on 700 .. 1500 keys, 32 / 8 heads of 128, bf16, 119 us, 600
+// TFLOP/s (154 us through registers); inside a long piece about 870.
 template <int DT, int D>
 __global__ __launch_bounds__((PrefillShape<DT, D, true>::kThreads)) void rows_wide_kernel(
     RowArgs a, const int32_t* __restrict__ bt) {

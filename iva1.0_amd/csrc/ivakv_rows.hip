@@ -24,6 +24,10 @@
 //
 // Bound: the K and V bytes of the shared pages, read once for up to 16 NR rows, and of the own
 // pages; from a few hundred rows on the matrix and vector pipes (4 D operations per key and row).
+// Measured per call, 32 / 8 heads of 128: 16 rows behind 8192 shared tokens (fp16, 50 MB) 19.3 us; 9
+// ragged groups (bf16, 277 MB) 71 us, 3.9 TB/s; 64 rows behind 4000 tokens on FP8 pages (149 MB) 53 us;
+// 256 rows behind 16384 120 us; beams of 5 rows on 16 sequences of 301 .. 1500 keys (60 MB) 18.3 us.  16
+// heads of 64: 16 sequences of 97 .. 448 rows on 700 .. 1500 keys 40 us, 445 TFLOP/s, by the vector pipe.
 #include <type_traits>
 
 #include "ivakv_rows.h"
@@ -919,11 +923,11 @@ struct Plan {
 // the waves' own registers in chunks of 32.  It reads the pages from the L2 once for eight times the
 // rows, but leaves a partial of all rows per piece and has one workgroup per CU to hide a piece's
 // start and end.  So it takes cross attention where whole chunks need no cutting into pieces (bf16,
-// D 128, walk : wide in us: 8 sequences of 200 x 2000, 32 / 8 heads 105 : 79, 16 of 97 .. 448 x 700 ..
-// 1500 200 : 151; cut in two, 16 of 64 x 1000 .. 1500 57 : 73), and a prefix long for its rows (bf16, 768 rows on
-// 8192 tokens 81 : 69, 1024 on 16384 155 : 128; 512 on 8192 49 : 57, 1024 on 2048 47 : 58).  At head_dim
-// 64 the softmax bounds both (16 of 448 x 1500, 16 heads 79 : 87).  FP8 pages would be rounded to the
-// queries' type on the way.
+// D 128, walk : wide in us: 8 sequences of 200 x 2000, 32 / 8 heads 100 : 73, 16 of 97 .. 448 x 700 ..
+// 1500 154 : 119, 16 of 300 x 1000 .. 1500, 16 heads 114 : 99; cut in two, 16 of 64 x 1000 .. 1500 50 :
+// 71), and a prefix long for its rows (768 rows on 8192 tokens 77 : 68, 1024 on 16384 155 : 128; 512 on
+// 8192 48 : 57, 1024 on 2048 47 : 58).  At head_dim 64 the softmax bounds both (16 of 448 x 1500, 16
+// heads 79 : 87).  FP8 pages would be rounded to the queries' type on the way.
 bool wide_walk(int head_dim, int dtype, bool fp8, bool prefix, int n_groups, int64_t rows, int hkv, int max_blocks) {
   if (fp8 || dtype == IVAKV_F32 || head_dim < 128 || rows < 256) return false;
   const int64_t chunk = wide_rows(head_dim);
