@@ -588,7 +588,9 @@ class PagedAttention(_AttentionBase):
         b, s, _ = x.shape
         returned = kv_cache
         cross = (not self.causal and key_ok is None and not (sliding_window and sliding_window > 0)
-                 and _plain_type(x) and _plain_mode() and b * s)
+                 and _plain_type(x) and _plain_mode() and b * s and self.head_dim in (64, 128, 256)
+                 and (kv_cache is None or (kv_cache.pool.block_size == 16
+                                           and (kv_cache.pool.fp8 or kv_cache.pool.dtype is x.dtype))))
         if kv_cache is None and (self.causal or cross):
             if x.is_cuda and b * s:
                 kv_cache = OwnPages(b, s, self.n_kv_heads, self.head_dim, x.device, x.dtype)
@@ -1056,6 +1058,8 @@ class Transformer(nn.Module):
         own_cache = kwargs.get("kv_cache") is None
         cache = kwargs.get("kv_cache") or self.new_kv_cache(batch_size, prompt_len + max_length,
                                                             samples=samples, prompt_len=prompt_len)
+        if samples > 1 and not hasattr(cache, "fork"):
+            raise ValueError(f"num_samples needs a cache that can be forked, got {type(cache).__name__}")
         use_graph = bool(kwargs.get("use_graph", False))
         if use_graph and not isinstance(cache, PagedKVCache):
             raise ValueError("use_graph needs attn_impl='hip_paged'")

@@ -140,6 +140,17 @@ def test_score_and_samples_on_the_cpu(M):
         model.generate(ids, num_samples=0)
 
 
+def test_samples_need_a_cache_that_forks(M):
+    cfg = M.TransformerConfig(d_model=32, n_layers=1, n_heads=2, vocab_size=40, seq_len=64, dropout=0.0)
+    model = M.Transformer(cfg).eval()
+
+    class Cache:  # (refused before the prompt runs through it)
+        seq_len = 0
+
+    with pytest.raises(ValueError, match="forked"):
+        model.generate(torch.zeros(1, 4, dtype=torch.long), max_length=3, num_samples=2, kv_cache=Cache())
+
+
 def test_logprobs_formula_masks(M):
     z = torch.tensor([[0.0, float("-inf"), 1.0], [2.0, 2.0, 2.0]])
     r = M._logprobs_of(z, torch.tensor([2, -100]), 2)

@@ -116,3 +116,22 @@ def test_non_causal_attention(M, dev, dtype, cached):
         got = both()
     ref = both().detach()  # (gradients on: the torch evaluation)
     assert (got.float() - ref.float()).abs().max() <= {torch.float16: 2e-3, torch.bfloat16: 1.6e-2}[dtype]
+
+
+@pytest.mark.parametrize("kw", [{"d_model": 128}, {"kv_block_size": 32}, {"d_model": 128, "kv_block_size": 8}], ids=str)
+def test_non_causal_attention_of_other_geometries(M, dev, kw):
+    """Head dims and page sizes that the kernel does not take: through torch, with a cache and
+    without, as under autograd."""
+    model = model_of(M, dev, dtype=torch.float16, causal=False, **kw)
+    attn = model.blocks[0].attention
+    width = kw.get("d_model", 256)
+    x = (torch.randn(2, 21, width, generator=torch.Generator().manual_seed(6)) * 0.5).to(dev, torch.float16)
+
+    def both():
+        cache = model.new_kv_cache(2, 21)
+        cache.num_layers = 1
+        return torch.cat([attn(x[:, :13], kv_cache=cache)[0], attn(x[:, 13:], kv_cache=cache)[0], attn(x)[0]], dim=1)
+
+    with torch.no_grad():
+        got = both()
+    assert (got.float() - both().detach().float()).abs().max() <= 2e-3

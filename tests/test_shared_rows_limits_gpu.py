@@ -155,3 +155,21 @@ def test_calls_from_threads_on_their_own_streams(iva, dev):
         th.join()
     for a, b in zip(got, want):
         assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("starts,prefixes,most", [([0], [], 0), ([2, 2], [64], 0), ([0, 5], [0], 5), ([1, 3, 3, 5], [64, 48, 64], 1)],
+                         ids=["no-groups", "empty-group", "empty-prefix", "past-max-group"])
+def test_rows_of_no_shared_walk(iva, dev, starts, prefixes, most):
+    """Rows of no group, of a group without a prefix, and past max_group read all of their pages
+    themselves: plain decode attention (fp16: the results' and P's half steps of values below 6,
+    twice)."""
+    gen = torch.Generator().manual_seed(4)
+    ks, vs = iva.pool_shapes(40, 2, 64, 16, torch.float16)
+    pools = [torch.randn(s, generator=gen).to(dev, torch.float16) for s in (ks, vs)]
+    bt = torch.cat([torch.arange(4).expand(5, 4), 4 + torch.arange(15).view(5, 3)], dim=1).int().contiguous().to(dev)
+    lens = torch.tensor([65, 112, 80, 64, 99], dtype=torch.int32, device=dev)
+    q = torch.randn(5, 8, 64, generator=gen).to(dev, torch.float16)
+    got = iva.paged_prefix_decode_attention(q, *pools, bt, lens, torch.tensor(starts, dtype=torch.int32, device=dev),
+                                            torch.tensor(prefixes, dtype=torch.int32, device=dev), max_group=most)
+    want = iva.paged_decode_attention(q, *pools, bt, lens)
+    assert (got.float() - want.float()).abs().max() <= 2 * 2 * 2.0 ** -11 * 6
