@@ -129,11 +129,11 @@ __device__ inline RowBlock row_block(const PrefillArgs& a, const int32_t* ctx, c
 }
 
 // Row block blk of (sequence b, kv head h) over pairs [pair_lo, pair_hi) of its walk
-// (pair_lo even).  kCausal false: every row sees all blk.L keys.  slot < 0: the block's whole walk, normalized rows into out; slot
-// >= 0: one segment of a split walk, its unnormalized rows (acc, running max, row sum)
-// into partial slot `slot` of the split workspace, for merge_rows.  Every
-// thread of the workgroup calls it with the same arguments (the returns and barriers
-// inside are uniform).
+// (pair_lo even).  kCausal false: every row sees all blk.L keys.  slot < 0: the block's
+// whole walk, normalized rows into out; slot >= 0: one segment of a split walk, its
+// unnormalized rows (acc, running max, row sum) into partial slot `slot` of the split
+// workspace, for merge_rows.  Every thread of the workgroup calls it with the same
+// arguments (the returns and barriers inside are uniform).
 template <int DT, int D, bool kFp8, bool kSplit, bool kCausal = true>
 __device__ __attribute__((always_inline)) inline void prefill_rows(
     const PrefillArgs& a, const int32_t* __restrict__ bt, const RowBlock& blk, int b, int h,
@@ -1028,11 +1028,13 @@ __global__ __launch_bounds__((PrefillShape<DT, D, true>::kThreads)) void prefill
     const int b = vu.x & 0xffff, h = vu.x >> 16, s = vu.y;
     const int2 rb = ws.rb[b * a.blocks_x + xb];
     if (s >= rb.y) continue;  // the block has no rows, or fewer segments
-    const RowBlock rows = row_block(a, ctx, qstart, b, xb, S::kRowsWG);
+    // (A row block for each walk: one for both costs the first walk's loop two waits, 1 %.)
     if (rb.y == 1) {
+      const RowBlock rows = row_block(a, ctx, qstart, b, xb, S::kRowsWG);
       prefill_rows<DT, D, kFp8, true>(a, bt, rows, b, h, 0, 0x7fffffff, -1);
       continue;
     }
+    const RowBlock rows = row_block(a, ctx, qstart, b, xb, S::kRowsWG);
     prefill_rows<DT, D, kFp8, true>(a, bt, rows, b, h, s * seg, (s + 1) * seg, rb.x + h * rb.y + s);
     // Count the segment in: every wave waits until its partial stores have reached this
     // XCD's L2 (the barrier alone waits only for LDS traffic), then thread 0's
