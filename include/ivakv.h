@@ -478,7 +478,7 @@ int ivakv_prefix_decode_attn(const void* q, const void* k_pool, const void* v_po
  * Rows of logits [n][vocab] (row_stride elements apart, each row dense): logprobs[i] = the log
  * probability of tokens[i] (0 where the token is outside [0, vocab): padding), entropy[i] in nats,
  * and the `top` most likely tokens in order (equal logits by index) with their log probabilities,
- * top <= min(vocab, 64).  A logit of -inf has probability 0; a row of nothing else has log
+ * top <= min(vocab, 64), n < 2^24.  A logit of -inf has probability 0; a row of nothing else has log
  * probabilities -inf and entropy 0; a NaN or +inf makes its row's results NaN (a NaN leads the
  * order).  stats ([n][2], may be NULL): what the gradient call needs.  Sums in fp32.
  * Replaces: log_softmax + gather over Transformer.forward's logits

@@ -34,6 +34,7 @@ constexpr float kLowest = -3.402823466e38f;
 // A difference z - m below this has weight 0 in fp32 (and keeps 0 * inf out of W).
 constexpr float kNoWeight = -1000.f;
 constexpr int kMaxTop = 64;
+constexpr int64_t kMaxRows = 0xffffff;  // (a grid has less than 2^32 threads, a row 256)
 
 struct LogprobArgs {
   const void* logits;
@@ -462,7 +463,7 @@ int check_logits(const char* name, const void* logits, int64_t stride, int64_t n
   if (n < 0 || vocab < 0 || stride < 0 || top < 0)
     return fail(IVAKV_E_ARG, "%s: bad sizes n=%lld vocab=%d stride=%lld top=%d", name, (long long)n, vocab,
                 (long long)stride, top);
-  if (n > 0x7fffffff) return fail(IVAKV_E_SHAPE, "%s: %lld rows", name, (long long)n);
+  if (n > kMaxRows) return fail(IVAKV_E_SHAPE, "%s: %lld rows, at most %lld", name, (long long)n, (long long)kMaxRows);
   if (top > kMaxTop || top > vocab)
     return fail(IVAKV_E_SHAPE, "%s: top %d exceeds %d", name, top, vocab < kMaxTop ? vocab : kMaxTop);
   if (n > 0 && vocab < 1) return fail(IVAKV_E_SHAPE, "%s: rows without logits", name);

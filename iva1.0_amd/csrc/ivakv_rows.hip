@@ -1051,8 +1051,12 @@ Plan plan_of(int n_groups, int n_rows, int num_q_heads, int num_kv_heads, int he
                    prefix ? (int64_t)n_rows * num_kv_heads * max_blocks : 0, max_blocks);
 }
 
-int check_plan(const char* name, const Plan& p, int num_kv_heads) {
-  if ((int64_t)p.items * num_kv_heads > 0x3fffffff)
+// Workgroups of a launch: with up to 512 threads each, a grid of less than 2^32 threads.
+constexpr int64_t kMaxGrid = 0x7fffff;
+
+int check_plan(const char* name, const Plan& p, int n_rows, int num_kv_heads, bool prefix) {
+  if ((int64_t)p.items * num_kv_heads + p.own_waves > kMaxGrid ||
+      ((prefix || p.split) && (int64_t)n_rows * num_kv_heads > kMaxGrid))
     return fail(IVAKV_E_SHAPE, "%s: launch too large", name);
   return IVAKV_OK;
 }
@@ -1087,7 +1091,7 @@ int rows_entry(const char* name, RowArgs a, int batch, int num_q_heads, int head
   a.max_rows = a.max_rows < a.n_rows ? a.max_rows : a.n_rows;
   const Plan p = plan_of(a.n_groups, a.n_rows, num_q_heads, a.Hkv, head_dim, a.max_rows, dtype, fp8,
                          a.max_blocks, a.prefix);
-  const int bad = check_plan(name, p, a.Hkv);
+  const int bad = check_plan(name, p, a.n_rows, a.Hkv, a.prefix);
   if (bad != IVAKV_OK) return bad;
   const Layout l = make_layout(p, a.n_rows, a.Hkv, a.G, head_dim);
   const size_t need = l.total * sizeof(float);
@@ -1120,7 +1124,7 @@ int workspace_size(const char* name, int n_groups, int n_rows, int num_q_heads, 
     return fail(IVAKV_E_ARG, "%s: bad sizes rows=%d max_blocks=%d", name, n_rows, max_blocks);
   const Plan p = plan_of(n_groups, n_rows, num_q_heads, num_kv_heads, head_dim,
                          max_rows < n_rows ? max_rows : n_rows, dtype, fp8, max_blocks, prefix);
-  const int bad = check_plan(name, p, num_kv_heads);
+  const int bad = check_plan(name, p, n_rows, num_kv_heads, prefix);
   if (bad != IVAKV_OK) return bad;
   *bytes = make_layout(p, n_rows, num_kv_heads, num_q_heads / num_kv_heads, head_dim).total * sizeof(float);
   return IVAKV_OK;

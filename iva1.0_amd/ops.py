@@ -940,7 +940,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0) -
 
     ``logits`` is ``[..., V]`` (float32, float16 or bfloat16), ``tokens`` integers of the leading
     shape.  A token outside ``[0, V)`` (padding, say -100) has log probability 0 and no gradient.
-    ``top_k`` <= min(V, 64); equal logits go by index.  A logit of -inf has probability 0; a row of
+    ``top_k`` <= min(V, 64); less than 2^24 rows; equal logits go by index.  A logit of -inf has probability 0; a row of
     nothing else has log probabilities -inf, entropy 0 and gradient 0; NaN or +inf in a row makes
     its results NaN.  Differentiable by the logits through ``logprobs``, ``entropy`` and
     ``top_logprobs`` (once).

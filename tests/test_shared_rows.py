@@ -119,6 +119,16 @@ def test_logprob_entry_refusals(iva, name, build):
     assert call(iva, name, *build(iva, n=0, logits=None, tokens=None, h=None)) == a.OK
 
 
+def test_launches_past_the_grid_are_refused(iva):
+    """A grid has less than 2^32 threads."""
+    a = iva._abi
+    for name, build in (("ivakv_token_logprobs", logprob_args), ("ivakv_token_logprobs_grad", grad_args)):
+        assert call(iva, name, *build(iva, n=1 << 24)) == a.E_SHAPE and str((1 << 24) - 1) in a.last_error()
+    # (cut into pieces: a join of every row and kv head)
+    assert call(iva, "ivakv_cross_attn", *cross_args(iva, n_tok=1 << 22, hq=4, hkv=4, max_q=1)) == a.E_SHAPE
+    assert call(iva, "ivakv_cross_attn", *cross_args(iva, n_tok=1 << 28, hq=4, hkv=4, max_q=1 << 28)) == a.E_SHAPE
+
+
 class _Device:
     """Stands for a GPU tensor in the ops' argument checks."""
     is_cuda, device, requires_grad = True, torch.device("cuda", 0), False
