@@ -517,8 +517,9 @@ class PagedAttention(_AttentionBase):
     one-layer paged cache of its own tokens, and None is returned, as the reference
     returns (attention.py:74-75).  Non-causal attention (``config.causal`` False) runs
     ivakv_cross_attn over the pages at inference on 16-bit tensors, and torch on the gathered
-    pages otherwise.  Decode steps of sequences forked from one prompt (PagedKVCache.fork) read the
-    pages they share once (ivakv_prefix_decode_attn) where that pays.  With a sliding window, once the forward's last layer is enqueued the cache releases the
+    pages otherwise.  Decode steps of sequences forked from one prompt (PagedKVCache.fork)
+    read the pages they share once (ivakv_prefix_decode_attn) where that pays.  With a
+    sliding window, once the forward's last layer is enqueued the cache releases the
     pages no later query can see (:meth:`PagedKVCache.release_window`; the sink pages
     stay resident), so a long sequence holds about window + sinks tokens per layer.
     A padding mask (``attention_mask`` with zeros, src/core/attention.py:95-97) is applied
