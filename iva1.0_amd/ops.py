@@ -934,6 +934,20 @@ class _TokenLogprobs(torch.autograd.Function):
         return grad, None, None
 
 
+def _same_stream_as_before(leaf: torch.Tensor, dev: torch.device):
+    """The leaf's gradient node, to be held until a graph holds it, with the stream it was made on
+    noted.  Refuses a capture whose backward pass would end in a gradient node that an eager graph of
+    the same leaf, still alive, made on another stream: autograd makes that stream wait for the
+    captured one, which breaks the capture and can end the process."""
+    node = torch.autograd.graph.get_gradient_edge(leaf).node
+    stream = _raw_stream(dev.index)
+    if node.metadata.setdefault("iva_stream", stream) != stream and _capturing(dev):
+        del node  # (not kept by the error's traceback)
+        raise RuntimeError("these logits have a live eager graph from another stream; drop its results "
+                           "before capturing their gradient")
+    return node
+
+
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0) -> TokenLogprobs:
     """Log probabilities of given tokens under rows of logits, with each row's entropy and its
     ``top_k`` most likely tokens, in one pass over the logits.
@@ -943,7 +957,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0) -
     ``top_k`` <= min(V, 64); less than 2^24 rows; equal logits go by index.  A logit of -inf has probability 0; a row of
     nothing else has log probabilities -inf, entropy 0 and gradient 0; NaN or +inf in a row makes
     its results NaN.  Differentiable by the logits through ``logprobs``, ``entropy`` and
-    ``top_logprobs`` (once).
+    ``top_logprobs`` (once).  A backward pass may be captured with its forward pass, while no
+    eager graph of the same leaves from another stream is alive.
 
     Replaces ``log_softmax`` and a gather over ``Transformer.forward``'s logits
     (src/core/transformer.py:242-255).
@@ -967,7 +982,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0) -
     flat = tokens if tokens.dim() == 1 else tokens.reshape(-1)
     flat = flat.to(torch.int64).contiguous()
     if (torch.is_grad_enabled() and logits.requires_grad) or fwAD._current_level >= 0:
+        # (held until the graph does: a node that dies in between would take its note along)
+        node = _same_stream_as_before(logits, dev) if logits.is_leaf and logits.requires_grad else None
         out = _TokenLogprobs.apply(rows, flat, top_k)
+        del node
     else:
         out = _token_logprobs(rows, flat, top_k, None)
     if len(lead) != 1:

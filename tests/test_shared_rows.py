@@ -178,3 +178,29 @@ def test_row_op_refusals(iva, op, what, change, error):
         else:
             iva.paged_prefix_decode_attention(q, kp, vp, bt, _Device(2, **i32), start, _Device(1, **i32), max_group=2,
                                               out=out)
+
+
+def test_capture_beside_a_live_eager_graph_is_refused(iva, monkeypatch):
+    """The check alone, on a leaf of the host with stand-ins for the stream and its state."""
+    ops, now = iva.ops, {"stream": 0, "capturing": False}
+    monkeypatch.setattr(ops, "_raw_stream", lambda index: now["stream"])
+    monkeypatch.setattr(ops, "_capturing", lambda dev: now["capturing"])
+    dev, leaf = torch.device("cuda", 0), torch.randn(2, 3, requires_grad=True)
+
+    def call():
+        node = ops._same_stream_as_before(leaf, dev)
+        out = leaf.sum()  # (holds the leaf's gradient node)
+        del node
+        return out
+
+    eager = call()
+    now.update(stream=7)
+    assert call() is not None  # another stream, but no capture
+    now.update(capturing=True)
+    with pytest.raises(RuntimeError, match="eager graph"):
+        call()
+    now.update(stream=0)
+    assert call() is not None  # the same stream
+    del eager
+    now.update(stream=7)
+    assert call() is not None  # the eager graph is gone

@@ -111,6 +111,41 @@ def test_logprobs_have_no_forward_gradient(iva, dev):
     assert graded.logprobs.requires_grad and not graded.top_tokens.requires_grad and not want.logprobs.requires_grad
 
 
+def test_logprobs_capture_beside_a_live_eager_graph(iva, dev):
+    """Refused while the eager results of the same leaf live; once they are dropped, captured,
+    replayed and right."""
+    leaf = torch.randn(4, 50, generator=torch.Generator().manual_seed(5)).to(dev).requires_grad_()
+    t, other = torch.arange(4, device=dev), torch.zeros(8, device=dev)
+    eager = iva.token_logprobs(leaf, t, 2)
+    stream = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        other.add_(1)
+        with pytest.raises(RuntimeError, match="eager graph"):
+            iva.token_logprobs(leaf, t, 2)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert other.sum() == 8
+    want = torch.autograd.grad((eager.logprobs + eager.entropy).sum(), leaf)[0]  # (the eager graph still works)
+    del eager
+    torch.cuda.synchronize()
+
+    def both():
+        r = iva.token_logprobs(leaf, t, 2)
+        return torch.autograd.grad((r.logprobs + r.entropy).sum(), leaf)[0]
+
+    with torch.cuda.stream(stream):
+        both()
+        again = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(again, stream=stream):
+            got = both()
+    for _ in range(2):
+        got.zero_()
+        again.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
 def test_calls_from_threads_on_their_own_streams(iva, dev):
     """Each thread's workspace is its stream's: as called alone, bit for bit."""
     def inputs(seed):
